@@ -463,6 +463,117 @@ int rh_kv_gather_to_host(const void* kpool, const void* vpool, const int* blocks
 int rh_kv_scatter_from_host(void* kpool, void* vpool, const int* blocks, int n, size_t block_bytes, const void* buf,
                             void* stream);
 
+/* ---- a decode step that stays on the device ------------------------------------------- */
+
+/* Four operators for programs that keep their batch on the device and capture its decode step
+ * into a graph: nothing of a step has to pass through the host. None of them has a counterpart
+ * in relay's CUDA code (relay builds tables on the host, block_manager.cpp, samples there,
+ * sampler.cpp, and reads a shared block once per sequence). The stream's device must be the
+ * current one, as for every launcher here. They allocate nothing and may be captured; calls
+ * that share a workspace, two captured graphs among them, must not overlap in time. */
+
+/* Block tables and slot maps of a step, from the lengths of its sequences.
+ *  cached [n_seqs]      tokens of each sequence that the cache holds
+ *  fresh  [n_seqs]      tokens that this step adds (0: the sequence waits)
+ *  shared [n_seqs]      leading keys that its group shares (NULL: none)
+ *  group_seqs [n_groups][2]  first sequence and number of sequences of each group
+ *  tables [n_seqs][table_stride]  block ids; sequence s holds ceil(cached[s] / block_size) on
+ *                       entry and ceil((cached[s] + fresh[s]) / block_size) afterwards
+ *  free_blocks, free_count   a stack of free ids: the new ones are free_blocks[*free_count - 1],
+ *                       free_blocks[*free_count - 2] and so on, in the order of the sequences
+ * and, written by the call, with one row per token, sequence after sequence:
+ *  row_off [n_seqs + 1] the rows of sequence s are row_off[s] .. row_off[s + 1] - 1
+ *  last_row [n_seqs]    its last row (0 if it waits): the rows of rh_rmsnorm, rh_gather_rows
+ *  table_off [n_seqs]   s * table_stride
+ *  pos, seq, slot [max_rows]  position, sequence and cache slot (block * block_size + slot in
+ *                       the block); rows past the step's tokens are idle: 0, 0 and -1
+ *  dec_meta [max_rows][4]     (row, position + 1, table offset, shared keys), 16-byte aligned;
+ *                       idle rows have context 0
+ *  groups [n_groups][4] (first row, rows, shared keys and table offset of its first sequence), 16-byte
+ *                       aligned: the groups of rh_shared_prefix_attention
+ *  totals [4]           tokens, ids taken, ids left on the stack, status
+ * cached, fresh and the stack are not written. free_count may be totals + 2, which carries the
+ * stack from step to step. A step that does not fit (status below, several of them added)
+ * takes no ids and has no rows: the tables stay as they are, every row is idle, the groups are
+ * empty. Lengths up to 2^30 - 2; n_seqs * table_stride below 2^31. */
+enum {
+  RH_STEP_ROWS_FULL = 1,  /* more than max_rows tokens */
+  RH_STEP_NO_BLOCKS = 2,  /* more blocks than the stack holds */
+  RH_STEP_TABLE_FULL = 4, /* a sequence past table_stride blocks */
+  RH_STEP_BAD_LENGTH = 8  /* a negative or too large length, a group that is no range of sequences */
+};
+int rh_step_tables(const int* cached, const int* fresh, const int* shared, int n_seqs, const int* group_seqs, int n_groups,
+                   int block_size, int* tables, int table_stride, const int* free_blocks, const int* free_count,
+                   int max_rows, int* row_off, int* last_row, int* table_off, int* pos, int* seq, int* slot,
+                   int* dec_meta, int* groups, int* totals, void* stream);
+
+/* rh_qkv_post_merge for models that normalise q and k per head: per token the sum of the
+ * product's planes (times scale if not NULL, plus bias if not NULL); per head x of q and k
+ * w * x / sqrt(mean(x^2) + eps) with w = q_norm or k_norm [head_dim], then RoPE (pairs (i, i + D/2),
+ * angle pos * inv_freq[i], the product in double precision, so that far positions keep theirs);
+ * q to q_out as fp16(q * q_scale), k and v as fp16 into the cache at slot[t] = block * block_size + slot
+ * in the block. A row with a negative slot is idle: nothing of it is read or written.
+ *  qkv     fp32 [planes][T][(heads + 2 kv_heads) head_dim], 16-byte aligned; planes = 1 is a plain
+ *          product, more are rh_gemm_w8_partials' (with its scale) or rh_gemm_f16_partials' ranges
+ *  q_out   fp16 [T][heads * head_dim], 8-byte aligned like the pools
+ * head_dim a multiple of 8, at most 512; planes at most 8. Two rows with one slot race. */
+int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T, const float* bias, const float* q_norm,
+                        const float* k_norm, float eps, const float* inv_freq, const int* pos, const int* slot,
+                        void* kpool, void* vpool, void* q_out, float q_scale, int heads, int kv_heads, int head_dim,
+                        int block_size, void* stream);
+
+/* rh_paged_decode_attention for tokens whose sequences share a prefix, whose keys are read once
+ * for all members of a group.
+ *  dec_meta [n_dec][4]   per token: its row in q and out, its context length, the offset of its
+ *                        block table in `tables`, how many leading keys its group shares
+ *  groups [n_groups][4]  first token, members (consecutive tokens of dec_meta), shared keys, offset
+ *                        of the table that the shared keys are read through
+ * A token attends to keys 0 .. context - 1: those below its shared keys through its group's table,
+ * the others through its own. It belongs to exactly one group if its shared keys are positive, and
+ * they are the group's; its context may end before them. A token of context 0 is idle, its row
+ * left as it was. Several tokens of one sequence are several entries.
+ *  max_members, max_shared, max_own  the largest group, the most shared keys and the most keys
+ *                        behind them: they choose how the work is cut. Beyond them results stay
+ *                        right and the call gets slower
+ *  workspace             rh_shared_prefix_workspace bytes for the same arguments, 16-byte aligned, all
+ *                        zero before its first call (each call leaves what the next needs)
+ * q, pools, tables, scale, out, head sizes and block sizes as for rh_paged_decode_attention. */
+int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, const void* kpool, const void* vpool,
+                               const int* dec_meta, const int* groups, const int* tables, int n_dec, int n_groups,
+                               int max_members, int max_shared, int max_own, int heads, int kv_heads, int head_dim,
+                               int block_size, float scale, void* workspace, size_t workspace_bytes, void* out,
+                               int64_t out_row_stride, void* stream);
+size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_members, int max_shared, int max_own, int heads,
+                                  int kv_heads, int head_dim);
+
+/* Penalties, biases and grammar masks on logits, and the greedy token of each row. For token v of
+ * row r, each step rounded to fp32:
+ *   seen in the row's history:        x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   count > 0 times in its output:    x = x - frequency[r] * count - presence[r]
+ *   named by its biases:              x = x + value (the last one, if several name it)
+ *   not allowed by its mask:          x = -inf
+ *  logits [rows] rows ld apart, out [rows] rows out_ld apart; out may be logits (with one ld)
+ *  history               row r: the first history_len[r] tokens at history + r * history_stride, of
+ *                        which the first prompt_len[r] (NULL: none) are the prompt and the rest the
+ *                        output; NULL: no penalties. Tokens outside 0 .. vocab - 1 count for nothing
+ *  repetition, frequency, presence [rows]  NULL: 1, 0, 0
+ *  bias_tokens, bias_values  row r: the first bias_len[r] at r * bias_stride; NULL: none
+ *  masks                 rows of bits mask_stride words apart (bit v % 32 of word v / 32: token v is
+ *                        allowed); row r uses mask mask_of[r], none where that is negative, and
+ *                        mask r where mask_of is NULL; NULL: no masks
+ *  next [rows]           the lowest token of the greatest result (NaN aside), -1 where none is above
+ *                        -inf; NULL: not wanted
+ *  workspace             only for next: rh_process_logits_workspace bytes, 8-byte aligned, all zero before
+ *                        its first call; each call leaves it all zero, so calls of other sizes
+ *                        may share it
+ * Lengths are taken as 0 below 0 and as the stride above it. */
+int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, const int* history, int64_t history_stride,
+                      const int* history_len, const int* prompt_len, const float* repetition, const float* frequency,
+                      const float* presence, const int* bias_tokens, const float* bias_values, int64_t bias_stride,
+                      const int* bias_len, const uint32_t* masks, int64_t mask_stride, const int* mask_of, float* out,
+                      int64_t out_ld, int* next, void* workspace, size_t workspace_bytes, void* stream);
+size_t rh_process_logits_workspace(int rows, int vocab);
+
 /* Fills out[i] (i < n) with fp16 / fp32 draws of mean + std * N(0, 1) from the
  * counter-based generator of rh_synth_normal_f32 (seed, stream, counter i). */
 int rh_fill_normal_f16(void* out, size_t n, uint64_t seed, uint64_t stream_id, float mean, float std, void* stream);

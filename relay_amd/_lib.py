@@ -112,6 +112,12 @@ SIGNATURES = {
     "rh_kv_scatter": (I, [P, P, P, I, SZ, P, P]),
     "rh_kv_gather_to_host": (I, [P, P, P, I, SZ, P, P]),
     "rh_kv_scatter_from_host": (I, [P, P, P, I, SZ, P, P]),
+    "rh_step_tables": (I, [P, P, P, I, P, I, I, P, I, P, P, I, P, P, P, P, P, P, P, P, P, P]),
+    "rh_qk_norm_to_cache": (I, [P, I, P, I, P, P, P, F, P, P, P, P, P, P, F, I, I, I, I, P]),
+    "rh_shared_prefix_attention": (I, [P, I64, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, SZ, P, I64, P]),
+    "rh_shared_prefix_workspace": (SZ, [I, I, I, I, I, I, I, I]),
+    "rh_process_logits": (I, [P, I64, I, I, P, I64, P, P, P, P, P, P, P, I64, P, P, I64, P, P, I64, P, P, SZ, P]),
+    "rh_process_logits_workspace": (SZ, [I, I]),
     "rh_fill_normal_f16": (I, [P, SZ, U64, U64, F, F, P]),
     "rh_fill_normal_f32": (I, [P, SZ, U64, U64, F, F, P]),
     "rh_synth_normal_f32": (None, [P, SZ, U64, U64, F, F]),

@@ -125,6 +125,25 @@ __device__ __forceinline__ float coherent_load(const float* p) {
   return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// ---- the raw partial planes of a split product -------------------------------------------
+
+constexpr int kMaxMergeSplit = 8;
+
+// The merged, scaled values of elements (t, n .. n + 3) (beta = 0: `+ 0.0f` keeps the
+// merge's sign of a zero result); every partial's 16-byte load issued before the adds.
+__device__ __forceinline__ float4 merged4(const float* ws, int ksn, int64_t plane, int64_t e, const float* sc) {
+  float4 p[kMaxMergeSplit];
+#pragma unroll
+  for (int z = 0; z < kMaxMergeSplit; ++z)
+    p[z] = z < ksn ? *reinterpret_cast<const float4*>(ws + z * plane + e) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+  float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int z = 0; z < kMaxMergeSplit; ++z)
+    if (z < ksn) v = float4{v.x + p[z].x, v.y + p[z].y, v.z + p[z].z, v.w + p[z].w};
+  if (!sc) return v;
+  return float4{mul_rounded(v.x, sc[0]), mul_rounded(v.y, sc[1]), mul_rounded(v.z, sc[2]), mul_rounded(v.w, sc[3])};
+}
+
 }  // namespace relay_hip
 
 // ---- host-side error plumbing for the C ABI ------------------------------------------

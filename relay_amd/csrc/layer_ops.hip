@@ -156,23 +156,6 @@ __global__ void gather_rows_kernel(const V* x, int nx, const V* a, int na, const
 // order); these kernels do that merge for the product's consumer in the same launch, with
 // the same arithmetic, so that a decode step saves the merge launch (~4.5 us at T = 32).
 
-constexpr int kMaxMergeSplit = 8;
-
-// The merged, scaled values of elements (t, n .. n + 3) (beta = 0: `+ 0.0f` keeps the
-// merge's sign of a zero result); every partial's 16-byte load issued before the adds.
-__device__ __forceinline__ float4 merged4(const float* ws, int ksn, int64_t plane, int64_t e, const float* sc) {
-  float4 p[kMaxMergeSplit];
-#pragma unroll
-  for (int z = 0; z < kMaxMergeSplit; ++z)
-    p[z] = z < ksn ? *reinterpret_cast<const float4*>(ws + z * plane + e) : float4{0.0f, 0.0f, 0.0f, 0.0f};
-  float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-  for (int z = 0; z < kMaxMergeSplit; ++z)
-    if (z < ksn) v = float4{v.x + p[z].x, v.y + p[z].y, v.z + p[z].z, v.w + p[z].w};
-  if (!sc) return v;
-  return float4{mul_rounded(v.x, sc[0]), mul_rounded(v.y, sc[1]), mul_rounded(v.z, sc[2]), mul_rounded(v.w, sc[3])};
-}
-
 // act = silu(gate) * up of the merged gate_up product (rows [0, I) gate, [I, 2I) up), the
 // arithmetic of silu_mul_vec_kernel; 8 elements per thread.
 __global__ void w8_merge_silu_kernel(const float* __restrict__ ws, int ksn, int T, int I,
