@@ -14,17 +14,25 @@
 // slices of a row are joined by log-sum-exp in a second launch.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "../../include/relay_hip.h"
 #include "common.h"
+#include "lds_ring.h"
+#ifndef RH_T1
+#define RH_T1 512
+#define RH_T2 512
+#endif
 
 namespace relay_hip {
 namespace {
 
-constexpr int kRows = 32;   // query rows of a workgroup
+constexpr int kStrip = 32;  // query rows of a wave: a strip
 constexpr int kStep = 32;   // keys of a wave's step
-constexpr int kWaves = 8;
+constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
+constexpr int kFew = 16;   // query rows of a workgroup whose waves take keys of their own
+constexpr int kRing = 4;    // 32-key tiles of K and V in LDS, where strips share them
 
 struct SharedArgs {
   const half_t* q;
@@ -35,7 +43,7 @@ struct SharedArgs {
   const int* tables;
   int n_dec, n_groups, heads, kv_heads, group, block, bs_shift;
   int shared_slice, shared_parts, own_slice, own_parts, tiles, own_tiles;  // tiles: row tiles of a group, of a token
-  int shared_wgs;                                                          // workgroups on prefixes, the first ones
+  int shared_units, shared_wgs, own_units;  // workgroups on prefixes come first
   float scale_log2;
   float *part_o, *part_ml;
   half_t* out;
@@ -53,239 +61,609 @@ __device__ __forceinline__ float row_max(float x) {
 }
 __device__ __forceinline__ float row_sum(float x) { return x + __shfl_xor(x, 32); }
 
-// Swizzle of a key's 16-byte chunks in the V staging rows.
+// Swizzle of a key's 16-byte chunks in LDS rows of K and V (flash_prefill.hip's, by the same reads).
 template <int D>
-__device__ __forceinline__ int vswz(int key) {
+__device__ __forceinline__ int kswz(int key) {
   return D == 128 ? ((key & 3) << 2) | ((key >> 2) & 3) : D == 64 ? key & 7 : (key >> 2) & 3;
 }
 
-// D: compute width, DR: head size of the rows (16 runs at width 32 with zeros behind).
-template <int D, int DR>
-__global__ __launch_bounds__(kThreads) void shared_attention_kernel(const SharedArgs a) {
-  constexpr int CH = D / 8;             // 16-byte chunks a row
-  constexpr int MK = D / 16;            // QK products a step
-  constexpr int DT = D / 32;            // 32-wide tiles of O^T
-  constexpr int VL = kStep * CH / kWave;
-  constexpr int XWAVE = DT * 16 * 64 + 2 * 64;  // floats that a wave hands over
-  constexpr int SMEM = std::max(kWaves * kStep * D * 2, kWaves / 2 * XWAVE * 4);
-  __shared__ __attribute__((aligned(16))) char smem[SMEM];
+// A strip's state in one wave: lanes c and c + 32 hold row c.
+template <int D>
+struct Strip {
+  float16v o[D / 32];
+  float ref, l;    // the row's offset in the log2 domain (-inf: no key seen), this lane's share of its sum
+  bool have_ref;   // wave-uniform: every row has one
+};
 
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int c = lane & 31, hh = lane >> 5;
-
-  // The workgroup's rows (as tokens and heads), table and keys.
-  int b = blockIdx.x, first, members, table_off, begin, end, part, tile, tile_step, kvh;
-  if (b < a.shared_wgs) {
-    tile = b % a.tiles, b /= a.tiles;
-    part = b % a.shared_parts, b /= a.shared_parts;
-    kvh = b % a.kv_heads;
-    const int4 g = a.groups[b / a.kv_heads];
-    first = g.x, members = g.y, table_off = g.w;
-    const int parts = parts_of(g.z, a.shared_slice, a.shared_parts);
-    if (part >= parts) return;
-    begin = part * a.shared_slice;
-    end = part == parts - 1 ? g.z : begin + a.shared_slice;
-    tile_step = a.tiles;
-  } else {
-    b -= a.shared_wgs;
-    tile = b % a.own_tiles, b /= a.own_tiles;
-    part = b % a.own_parts, b /= a.own_parts;
-    kvh = b % a.kv_heads;
-    first = b / a.kv_heads, members = 1;
-    const int4 m = a.meta[first];
-    table_off = m.z;
-    const int from = max(m.w, 0), parts = parts_of(m.y - from, a.own_slice, a.own_parts);
-    if (part >= parts) return;
-    begin = from + part * a.own_slice;
-    end = part == parts - 1 ? m.y : begin + a.own_slice;
-    part += parts_of(m.w, a.shared_slice, a.shared_parts);
-    tile_step = a.own_tiles;
+// P = exp2(S scale - ref), the sum and the offset. An offset moves only when a row's weights pass 2^15
+// (a lane's sum tells): O and l are rescaled on a few steps, not on all (64 multiplies a step at
+// head size 128). A masked key's S is -inf.
+template <int D>
+__device__ __forceinline__ void weigh(Strip<D>& st, const float16v& s, half8 (&p)[2], float scale) {
+  float sum = 0.0f;
+  const auto weights = [&](float nref) {
+    sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const float x = fast_exp2(fmaf(s[e], scale, nref));
+      sum += x;
+      p[e >> 3][e & 7] = static_cast<half_t>(x);
+    }
+  };
+  bool slow = !st.have_ref;
+  if (!slow) {
+    weights(-st.ref);
+    slow = __ballot(!(sum <= 32768.0f)) != 0;
   }
-  const int* table = a.tables + table_off;
-  const int G = a.group, bs = a.block, sh = a.bs_shift;
+  if (slow) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e] * scale);
+    mx = row_max(mx);
+    float alpha = 1.0f;
+    if (mx > st.ref + 8.0f || st.ref == -INFINITY) {
+      alpha = st.ref == -INFINITY ? 0.0f : fast_exp2(st.ref - mx);
+      st.ref = mx;
+    }
+    weights(st.ref == -INFINITY ? 0.0f : -st.ref);
+    st.l *= alpha;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) st.o[i][e] *= alpha;
+    st.have_ref = __ballot(st.ref == -INFINITY) == 0;
+  }
+  st.l += sum;
+}
 
-  for (; tile * kRows < members * G; tile += tile_step) {
-    const int r = tile * kRows + c;
-    const bool on = r < members * G;
-    const int token = first + (on ? r / G : 0), head = kvh * G + (on ? r % G : 0);
+// V^T operands of 32 keys whose rows begin at sv: a transposing read gives a lane rows kr .. kr + 3 of
+// its column (S^T's key order).
+template <int D>
+__device__ __forceinline__ void read_v(half8 (&v)[2][D / 32], const half_t* sv) {
+  const int lane = threadIdx.x & 63, hh = lane >> 5, i16 = lane & 15;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      const int col = 32 * i + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
+      const int kr = 16 * u + 4 * hh + (i16 >> 2);
+      const half4 a = tr_read_b64(sv + kr * D + (((col >> 3) ^ kswz<D>(kr)) << 3) + (col & 7));
+      const half4 b = tr_read_b64(sv + (kr + 8) * D + (((col >> 3) ^ kswz<D>(kr + 8)) << 3) + (col & 7));
+      v[u][i] = half8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+}
+
+// O^T += V^T P^T
+template <int D>
+__device__ __forceinline__ void add_pv(Strip<D>& st, const half8 (&v)[2][D / 32], const half8 (&p)[2]) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) st.o[i] = mfma32x32x16(v[u][i], p[u], st.o[i]);
+}
+
+// Only keys lo .. lim - 1 of the 32 from key0 on count. (The empty asm keeps the selects in the branch
+// that calls this: as selects on every step they cost 100 registers.)
+__device__ __forceinline__ void mask_keys(float16v& s, int key0, int lo, int lim) {
+  asm volatile("");
+  const int first = key0 + 4 * ((threadIdx.x & 63) >> 5), from = lo - first, to = lim - first;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int k = 8 * (e >> 2) + (e & 3);
+    if (k < from || k >= to) s[e] = -INFINITY;
+  }
+}
+
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// 1 KB from global memory to LDS: lane l's 16 bytes at base + offset go to lds + 16 l. No output
+// register; the ring's own waits order it before the reads (as lds_ring.h's buffer form, which
+// reaches 2 GB from its base; a cache may be larger).
+__device__ __forceinline__ void global_to_lds(const half_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(offset), "s"(base), "s"(lds)
+               : "memory");
+}
+
+// A workgroup's share: rows of `members` tokens' G heads (row tiles tile, tile + step, ...) against keys
+// begin .. end - 1 of a table.
+struct Share {
+  int first, members, kvh, begin, end, part, tile, step;
+  const int* table;
+};
+
+typedef const __attribute__((address_space(4))) int* scalar_ints;  // uniform reads go through the scalar unit
+
+// ---- many rows: the waves share tiles of K and V in LDS, 32 rows a wave ---------------------------
+//
+//   S^T[32 keys x 32 rows] = K[32 keys x D] * Q^T[D x 32 rows]          (MFMA 32x32x16)
+//   O^T[D x 32 rows] += V^T[D x 32 keys] * P^T[32 keys x 32 rows]       (MFMA 32x32x16)
+//
+// with lanes c and c + 32 on row c. Tiles come by loads straight to LDS into a ring of kRing, three
+// tiles ahead. D is the head size; 16 keys from a multiple of 16 on lie in one block.
+template <int D>
+__device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* smem) {
+  constexpr int CH = D / 8;            // 16-byte chunks a row
+  constexpr int MK = D / 16;           // QK products a step
+  constexpr int DT = D / 32;           // 32-wide tiles of O^T
+  constexpr int KEYS = kWave / CH;     // keys of a 1 KB piece
+  constexpr int PER16 = 16 / KEYS;     // pieces of 16 keys
+  constexpr int TILE = kStep * D;      // halves of a tile's K
+  static_assert(KEYS <= 16, "a piece lies in one block");
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.group, bs = a.block, sh = a.bs_shift;
+  const half_t* const ring = reinterpret_cast<const half_t*>(smem);
+  const uint32_t lds = __builtin_amdgcn_readfirstlane(lds_address(smem));
+  const scalar_ints entries = (scalar_ints)(g.table);
+  const half_t* const pool = w >= 2 ? a.vpool : a.kpool;
+  const int n = (g.end - g.begin + kStep - 1) / kStep;
+
+  for (; g.tile * kWaves * kStrip < g.members * G; g.tile += g.step) {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));  // keeps what depends on it from being held across the loop over tiles
+    const int c = lane & 31, hh = lane >> 5;
+    // A wave brings half a tile's K or V, 16 keys of one table entry, which it looks up a tile ahead.
+    int entry;
+    const auto first16 = [&](int j) { return min(g.begin + j * kStep + 16 * (w & 1), (g.end - 1) & ~15); };
+    const auto lookup = [&](int j) { entry = entries[first16(j) >> sh]; };
+    const auto send = [&](int j) {
+      const int key = first16(j);
+      const half_t* const base = pool + ((static_cast<int64_t>(entry) * a.kv_heads + g.kvh) * bs + (key & (bs - 1))) * D;
+      const int last = g.end - 1 - key;
+#pragma unroll
+      for (int i = 0; i < PER16; ++i) {
+        const int at = i * KEYS + lane / CH, k = 16 * (w & 1) + at;  // of the 16 keys, of the tile
+        const int cc = (lane % CH) ^ kswz<D>(k);
+        global_to_lds(base, (min(at, last) * D + 8 * cc) * 2,  // past the end: the last key again
+                      lds + (j % kRing * 2 * TILE + (w >> 1) * TILE + (16 * (w & 1) + i * KEYS) * D) * 2);
+      }
+    };
+    lookup(0);
+    for (int j = 0; j < kRing - 1; ++j)
+      if (j < n) {
+        send(j);
+        lookup(j + 1);
+      }
+
+    const int r = (g.tile * kWaves + w) * kStrip + c;
+    const bool on = r < g.members * G;
+    const int token = g.first + (on ? r / G : 0), head = g.kvh * G + (on ? r % G : 0);
     const int4 m = a.meta[token];
-    const int lim = on ? min(m.y, end) : 0;  // the row sees the keys before this
+    const int lim = on ? min(m.y, g.end) : g.end;  // the row sees the keys before this
+    int all = lim;                                 // every row of the strip sees the keys before this
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all = min(all, __shfl_xor(all, o));
+    all = __builtin_amdgcn_readfirstlane(all);
 
     half8 qb[MK];
 #pragma unroll
     for (int i = 0; i < MK; ++i) {
-      if (lim > 0 && (DR == D || 16 * i + 8 * hh < DR)) {
-        qb[i] = load_half8(a.q + m.x * a.q_stride + static_cast<int64_t>(head) * DR + 16 * i + 8 * hh);
+      if (on && m.y > 0) {
+        qb[i] = load_half8(a.q + m.x * a.q_stride + static_cast<int64_t>(head) * D + 16 * i + 8 * hh);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) qb[i][e] = 0;
       }
     }
-    float16v o[DT];
+#pragma unroll
+    for (int i = 0; i < MK; ++i) asm volatile("" : "+v"(qb[i]));  // q is here: the loop waits for its own loads alone
+    Strip<D> st;
+    st.ref = -INFINITY, st.l = 0.0f, st.have_ref = false;
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[i][e] = 0.0f;
-    float m_run = -INFINITY, l_run = 0.0f;
-    half_t* const sv = reinterpret_cast<half_t*>(smem) + w * kStep * D;
+      for (int e = 0; e < 16; ++e) st.o[i][e] = 0.0f;
 
-    const auto offset = [&](int key) {
-      key = min(key, end - 1);
-      const int blk = table[sh >= 0 ? key >> sh : key / bs];
-      return kv_row_offset(blk, a.kv_heads, kvh, bs, sh >= 0 ? key & (bs - 1) : key % bs, DR);
+    // Step j has S of tile j. It waits for tile j + 1 (one barrier, which also frees tile j - 1's
+    // buffer to be sent for again), reads its K while tile j's weights are computed, and tile j's V
+    // while the next S is: the LDS reads' latency lies under other work.
+    const auto tile_at = [&](int j) { return ring + j % kRing * 2 * TILE; };
+    half8 k[MK];
+    const auto read_k = [&](int j) {
+      const half_t* const kt = tile_at(j) + c * D;
+#pragma unroll
+      for (int i = 0; i < MK; ++i) k[i] = *reinterpret_cast<const half8*>(kt + (((2 * i + hh) ^ kswz<D>(c)) << 3));
     };
-    for (int k0 = begin + w * kStep; k0 < end; k0 += kWaves * kStep) {
-      half8 k[MK], v[VL];
-      const int64_t krow = offset(k0 + c);
-#pragma unroll
-      for (int i = 0; i < MK; ++i) {
-        if (DR == D || 16 * i + 8 * hh < DR) {
-          k[i] = load_half8(a.kpool + krow + 16 * i + 8 * hh);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) k[i][e] = 0;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < VL; ++i) {
-        const int kl = i * (kWave / CH) + lane / CH, cc = lane % CH;
-        if ((DR == D || 8 * cc < DR) && k0 + kl < end) {
-          v[i] = load_half8(a.vpool + offset(k0 + kl) + 8 * cc);
-        } else {  // its weight is 0, its bytes may be anything
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] = 0;
-        }
-        *reinterpret_cast<half8*>(sv + kl * D + ((cc ^ vswz<D>(kl)) << 3)) = v[i];
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-
-      float16v s;
+    float16v s;
+    const auto scores = [&] {
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = 0.0f;
 #pragma unroll
       for (int i = 0; i < MK; ++i) s = mfma32x32x16(k[i], qb[i], s);
-      float mx = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int key = k0 + 8 * (e >> 2) + 4 * hh + (e & 3);
-        s[e] = key < lim ? s[e] * a.scale_log2 : -INFINITY;
-        mx = fmaxf(mx, s[e]);
+    };
+    wait_stages<PER16, kRing - 2>(min(n - 1, kRing - 2));
+    ring_barrier();
+    const bool busy = (g.tile * kWaves + w) * kStrip < g.members * G;  // a wave without rows only brings tiles
+    read_k(0);
+    scores();
+    for (int j = 0; j < n; ++j) {
+      const bool more = j + 1 < n;
+      if (more) wait_stages<PER16, kRing - 3>(min(n - 2 - j, kRing - 3));
+      ring_barrier();
+      if (j + kRing - 1 < n) {
+        send(j + kRing - 1);
+        lookup(j + kRing);
       }
-      const float m_new = fmaxf(m_run, row_max(mx));
-      const float ref = m_new == -INFINITY ? 0.0f : m_new;
-      const float alpha = fast_exp2(m_run - ref);
-      m_run = m_new;
-      half8 p[2];
-      float sum = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float x = fast_exp2(s[e] - ref);
-        sum += x;
-        p[e >> 3][e & 7] = static_cast<half_t>(x);
-      }
-      l_run = l_run * alpha + sum;
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] *= alpha;
-      // V^T: a transposing read gives a lane rows kr .. kr + 3 of its column (S^T's key order).
-      const int i16 = lane & 15;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < DT; ++i) {
-          const int col = 32 * i + 16 * ((lane >> 4) & 1) + 4 * (i16 & 3);
-          const int kr = 16 * u + 4 * hh + (i16 >> 2);
-          const half4 lo = tr_read_b64(sv + kr * D + (((col >> 3) ^ vswz<D>(kr)) << 3) + (col & 7));
-          const half4 hi = tr_read_b64(sv + (kr + 8) * D + (((col >> 3) ^ vswz<D>(kr + 8)) << 3) + (col & 7));
-          o[i] = mfma32x32x16(half8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, p[u], o[i]);
-        }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      if (!busy) continue;
+      if (more) read_k(j + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      const int k0 = g.begin + j * kStep;
+      if (k0 + kStep > all) mask_keys(s, k0, g.begin, lim);
+      half8 p[2], v[2][DT];
+      weigh(st, s, p, a.scale_log2);
+      read_v<D>(v, tile_at(j) + TILE);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) scores();
+      add_pv(st, v, p);
     }
-    l_run = row_sum(l_run);
+    st.l = row_sum(st.l);
+    __syncthreads();
 
-    // The waves' halves join pairwise through LDS until the first holds the slice.
-    for (int n = kWaves / 2; n > 0; n >>= 1) {
-      __syncthreads();
-      float* const x = reinterpret_cast<float*>(smem) + (w % n) * XWAVE;
-      if (w >= n && w < 2 * n) {
+    // Out through LDS, so that a row's values leave as whole lines (each wave has 32 rows of D floats
+    // there; row c is rotated by 4 c: the 32 rows of one write would otherwise hit the same banks).
+    float* const x = reinterpret_cast<float*>(smem) + w * kStrip * D;
 #pragma unroll
-        for (int i = 0; i < DT; ++i)
+    for (int i = 0; i < DT; ++i)
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[(i * 16 + e) * 64 + lane] = o[i][e];
-        x[DT * 16 * 64 + lane] = m_run;
-        x[DT * 16 * 64 + 64 + lane] = l_run;
-      }
-      __syncthreads();
-      if (w < n) {
-        const float m2 = x[DT * 16 * 64 + lane], l2 = x[DT * 16 * 64 + 64 + lane];
-        const float mm = fmaxf(m_run, m2), ref = mm == -INFINITY ? 0.0f : mm;
-        const float f1 = fast_exp2(m_run - ref), f2 = fast_exp2(m2 - ref);
-        m_run = mm;
-        l_run = l_run * f1 + l2 * f2;
+      for (int e = 0; e < 16; e += 4)
+        *reinterpret_cast<float4*>(x + c * D + ((32 * i + 2 * e + 4 * hh + 4 * c) & (D - 1))) =
+            float4{st.o[i][e], st.o[i][e + 1], st.o[i][e + 2], st.o[i][e + 3]};
+    const int64_t at = on && m.y > 0 ? (static_cast<int64_t>(token) * a.heads + head) * (a.shared_parts + a.own_parts) + g.part : -1;
+    if (hh == 0 && at >= 0) reinterpret_cast<float2*>(a.part_ml)[at] = float2{st.ref, st.l};
+    wave_fence();
+    constexpr int LANES = D / 4, ROWS = kWave / LANES;  // lanes of a row, rows a store
 #pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[i][e] = o[i][e] * f1 + x[(i * 16 + e) * 64 + lane] * f2;
-      }
-    }
-    if (w == 0 && on && m.y > 0) {
-      const int64_t at = (static_cast<int64_t>(token) * a.heads + head) * (a.shared_parts + a.own_parts) + part;
-      if (hh == 0) {
-        a.part_ml[2 * at] = m_run;
-        a.part_ml[2 * at + 1] = l_run;
-      }
-#pragma unroll
-      for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-          const int d = 32 * i + 2 * e + 4 * hh;
-          if (DR == D || d < DR) *reinterpret_cast<float4*>(a.part_o + at * DR + d) = float4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
-        }
+    for (int i = 0; i < kStrip; i += ROWS) {
+      const int row = i + lane / LANES, d = 4 * (lane % LANES);
+      const int64_t to = __shfl(at, row);
+      const float4 v = *reinterpret_cast<const float4*>(x + row * D + ((d + 4 * row) & (D - 1)));
+      if (to >= 0) *reinterpret_cast<float4*>(a.part_o + to * D + d) = v;
     }
     __syncthreads();
   }
 }
 
-// A thread per output value.
-__global__ void shared_join_kernel(const SharedArgs a, int D) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= static_cast<int64_t>(a.n_dec) * a.heads * D) return;
-  const int d = static_cast<int>(i % D), head = static_cast<int>(i / D % a.heads), token = static_cast<int>(i / D / a.heads);
+// ---- few rows: the waves take steps of 32 keys of their own -----------------------------------------
+//
+//   S^T[16 keys x 16 rows] = K[16 keys x D] * Q^T[D x 16 rows], twice     (MFMA 16x16x32)
+//   O^T[D x 16 rows] += V^T[D x 32 keys] * P^T[32 keys x 16 rows]         (MFMA 16x16x32)
+//
+// with lane (c, g) on row c and keys 4 g .. 4 g + 3 of each 16. K goes straight into MFMA operands, V through a
+// staging area of the wave in LDS, and the loads of the next step are in flight under this one's work,
+// so that a workgroup alone on its CU, as at the end of a batch of ragged lengths, still streams.
+template <int D, int DR>
+struct KvStep {
+  half8 k[2][D / 32], v[kStep * (D / 8) / kWave];
+};
+
+// Swizzle of a key's 16-byte chunks in the staging rows.
+template <int D>
+__device__ __forceinline__ int vswz(int key) {
+  return D >= 64 ? ((key >> 2) & 3) << 1 : ((key >> 2) & 1) << 1;
+}
+
+template <int D, int DR, bool SCALAR>
+__device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* smem) {
+  constexpr int CH = D / 8, KH = D / 32, DT = D / 16, VL = kStep * CH / kWave, VKEYS = kWave / CH;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int G = a.group, bs = a.block, bshift = a.bs_shift, begin = sh.begin, end = sh.end;
+  const scalar_ints entries = (scalar_ints)(sh.table);
+  half_t* const sv = reinterpret_cast<half_t*>(smem) + w * kStep * D;
+  float* const s_ml = reinterpret_cast<float*>(smem + kWaves * kFew * D * 4);  // [wave][16 rows][max, sum]
+
+  for (; sh.tile * kFew < sh.members * G; sh.tile += sh.step) {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int c = lane & 15, g = lane >> 4;
+    const auto row_any = [&](int j) -> unsigned {
+      j = min(j, end - 1);
+      return (static_cast<unsigned>(sh.table[bshift >= 0 ? j >> bshift : j / bs]) * a.kv_heads + sh.kvh) * bs +
+             (bshift >= 0 ? j & (bs - 1) : j % bs);
+    };
+    // SCALAR: the table entries of the two 16-key runs of a step, looked up a step ahead. The first
+    // run may begin before `begin`, whose slots may hold anything: rows are clamped at both ends.
+    int entry[2];
+    const auto run_of = [&](int k0, int t) { return min(k0 + 16 * t, (end - 1) & ~15); };
+    const auto lookup = [&](int k0) {
+      if (SCALAR) entry[0] = entries[run_of(k0, 0) >> bshift], entry[1] = entries[run_of(k0, 1) >> bshift];
+    };
+    const auto issue = [&](KvStep<D, DR>& st, int k0) {
+      const auto row_of = [&](int t, int off) -> unsigned {
+        const int r0 = run_of(k0, t);
+        return (static_cast<unsigned>(entry[t]) * a.kv_heads + sh.kvh) * bs + (r0 & (bs - 1)) + min(max(off, begin - r0), end - 1 - r0);
+      };
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const half_t* const at = a.kpool + static_cast<int64_t>(SCALAR ? row_of(t, c) : row_any(k0 + 16 * t + c)) * DR;
+#pragma unroll
+        for (int h = 0; h < KH; ++h) {
+          if (DR == D || 32 * h + 8 * g < DR) {
+            st.k[t][h] = load_half8(at + 32 * h + 8 * g);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) st.k[t][h][e] = 0;
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const int kl = VKEYS * i;  // first key of the load
+        const half_t* const at = a.vpool + static_cast<int64_t>(SCALAR ? row_of(kl >> 4, (kl & 15) + lane / CH) : row_any(k0 + kl + lane / CH)) * DR;
+        if (DR == D || 8 * (lane % CH) < DR) {
+          st.v[i] = load_half8(at + 8 * (lane % CH));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) st.v[i][e] = 0;
+        }
+      }
+      lookup(k0 + kWaves * kStep);
+    };
+
+    const int r = sh.tile * kFew + c;
+    const bool on = r < sh.members * G;
+    const int token = sh.first + (on ? r / G : 0), head = sh.kvh * G + (on ? r % G : 0);
+    int k0 = (SCALAR ? begin & ~15 : begin) + w * kStep;
+    KvStep<D, DR> ahead[2];
+    lookup(k0);
+    if (k0 < end) issue(ahead[0], k0);
+    const int4 m = a.meta[token];
+    const int lim = on ? min(m.y, end) : end;
+    half8 qb[KH];
+#pragma unroll
+    for (int h = 0; h < KH; ++h) {
+      if (on && m.y > 0 && (DR == D || 32 * h + 8 * g < DR)) {
+        qb[h] = load_half8(a.q + m.x * a.q_stride + static_cast<int64_t>(head) * DR + 32 * h + 8 * g);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) qb[h][e] = 0;
+      }
+    }
+    float ref = -INFINITY, l = 0.0f;
+    float4v o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i) o[i] = float4v{0.0f, 0.0f, 0.0f, 0.0f};
+
+    const auto compute = [&](const KvStep<D, DR>& st) {
+#pragma unroll
+      for (int i = 0; i < VL; ++i) {
+        const int kl = VKEYS * i + lane / CH;
+        *reinterpret_cast<half8*>(sv + kl * D + (((lane % CH) ^ vswz<D>(kl)) << 3)) = st.v[i];
+      }
+      float x[8], mx = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < KH; ++h) s = mfma16x16x32(st.k[t][h], qb[h], s);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = k0 + 16 * t + 4 * g + e;
+          x[4 * t + e] = key >= begin && key < lim ? s[e] * a.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, x[4 * t + e]);
+        }
+      }
+      mx = fmaxf(ref, group4_max(mx));
+      const float base = mx == -INFINITY ? 0.0f : mx, alpha = fast_exp2(ref - base);
+      ref = mx;
+      half8 p;
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = fast_exp2(x[e] - base);
+        sum += y;
+        p[e] = static_cast<half_t>(y);
+      }
+      l = l * alpha + sum;
+      wave_fence();
+#pragma unroll
+      for (int i = 0; i < DT; ++i) {
+        // A transposing read gives lane c of group g rows kr .. kr + 3 of column 16 i + c.
+        const int col = 16 * i + 4 * (c & 3), kr = 4 * g + (c >> 2);
+        const half4 lo = tr_read_b64(sv + kr * D + (((col >> 3) ^ vswz<D>(kr)) << 3) + (col & 7));
+        const half4 hi = tr_read_b64(sv + (kr + 16) * D + (((col >> 3) ^ vswz<D>(kr + 16)) << 3) + (col & 7));
+        float4v acc = o[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] *= alpha;
+        o[i] = mfma16x16x32(half8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}, p, acc);
+      }
+      wave_fence();
+    };
+    while (k0 < end) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (k0 < end) {
+          if (k0 + kWaves * kStep < end) issue(ahead[1 - i], k0 + kWaves * kStep);
+          __builtin_amdgcn_sched_barrier(0);  // the next step's loads before this one's arithmetic
+          compute(ahead[i]);
+          k0 += kWaves * kStep;
+        }
+      }
+    }
+    l = group4_sum(l);
+
+    // The waves' rows meet in LDS (row c rotated by 4 c floats against bank conflicts).
+    __syncthreads();
+    float* const so = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) so[(w * kFew + c) * D + ((16 * i + 4 * g + 4 * c) & (D - 1)) + e] = o[i][e];
+    if (g == 0) s_ml[2 * (w * kFew + c)] = ref, s_ml[2 * (w * kFew + c) + 1] = l;
+    __syncthreads();
+    const int rows = min(kFew, sh.members * G - sh.tile * kFew);
+    for (int i = threadIdx.x; i < rows * DR; i += kThreads) {
+      const int row = i / DR, d = i % DR, rr = sh.tile * kFew + row;
+      const int tk = sh.first + rr / G, hd = sh.kvh * G + rr % G;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < kWaves; ++j) top = fmaxf(top, s_ml[2 * (j * kFew + row)]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      float L = 0.0f, O = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kWaves; ++j) {
+        const float f = fast_exp2(s_ml[2 * (j * kFew + row)] - base);
+        L += f * s_ml[2 * (j * kFew + row) + 1];
+        O += f * so[(j * kFew + row) * D + ((d + 4 * row) & (D - 1))];
+      }
+      const int64_t at = (static_cast<int64_t>(tk) * a.heads + hd) * (a.shared_parts + a.own_parts) + sh.part;
+      a.part_o[at * DR + d] = O;  // an idle token's are never read
+      if (d == 0) reinterpret_cast<float2*>(a.part_ml)[at] = float2{top, L};
+    }
+    __syncthreads();
+  }
+}
+
+// D: compute width, DR: head size of the rows (16 runs at width 32 with zeros behind). SCALAR: the
+// block size is a power of two >= 16, so 16 keys from a multiple of 16 on lie in one block. ROWS: prefixes
+// have many rows.
+template <int D, int DR, bool SCALAR, bool ROWS>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D > 64 ? 2 : 3, D > 64 ? 2 : 4))) void shared_attention_kernel(
+    const SharedArgs a) {
+  constexpr int FEW = kWaves * kFew * (D * 4 + 8), RING = ROWS ? kRing * 2 * kStep * D * 2 : 0;
+  __shared__ __attribute__((aligned(16))) char smem[std::max(FEW, RING)];
+  static_assert(kWaves * kStep * D * 2 <= FEW && (!ROWS || kWaves * kStrip * D * 4 <= RING), "staging and hand-over fit");
+
+  // Workgroups go round the 8 XCDs; the row tiles of one slice share an XCD, whose L2 then holds its K and V.
+  const bool shared = blockIdx.x < static_cast<unsigned>(a.shared_wgs);
+  int b = shared ? blockIdx.x : blockIdx.x - a.shared_wgs;
+  Share g;
+  g.step = shared ? a.tiles : a.own_tiles;
+  g.tile = (b >> 3) % g.step;
+  b = (b >> 3) / g.step * 8 + (b & 7);
+  if (b >= (shared ? a.shared_units : a.own_units)) return;
+  if (shared) {
+    g.part = b % a.shared_parts, b /= a.shared_parts;
+    g.kvh = b % a.kv_heads;
+    const int4 rec = a.groups[b / a.kv_heads];
+    const int parts = parts_of(rec.z, a.shared_slice, a.shared_parts);
+    if (g.part >= parts) return;
+    g.first = rec.x, g.members = rec.y, g.table = a.tables + rec.w;
+    g.begin = g.part * a.shared_slice;
+    g.end = g.part == parts - 1 ? rec.z : g.begin + a.shared_slice;
+    if constexpr (ROWS) {
+      attend_rows<D>(a, g, smem);
+      return;
+    }
+  } else {
+    g.part = b % a.own_parts, b /= a.own_parts;
+    g.kvh = b % a.kv_heads;
+    g.first = b / a.kv_heads, g.members = 1;
+    const int4 m = a.meta[g.first];
+    const int from = max(m.w, 0), parts = parts_of(m.y - from, a.own_slice, a.own_parts);
+    if (g.part >= parts) return;
+    g.table = a.tables + m.z;
+    g.begin = from + g.part * a.own_slice;
+    g.end = g.part == parts - 1 ? m.y : g.begin + a.own_slice;
+    g.part += parts_of(m.w, a.shared_slice, a.shared_parts);
+  }
+  attend_few<D, DR, SCALAR>(a, g, smem);
+}
+
+// Joins a row's slices: D / 4 lanes a row, four values a lane. The lanes bring 32 slices' maxima and
+// sums at once, one or two each, and kJoin slices' values at once.
+constexpr int kJoin = 8;
+template <int D>
+__global__ __launch_bounds__(256) void shared_join_kernel(const SharedArgs a) {
+  constexpr int LANES = D / 4;
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+  if (row >= static_cast<int64_t>(a.n_dec) * a.heads) return;
+  const int token = static_cast<int>(row / a.heads), head = static_cast<int>(row % a.heads);
   const int4 m = a.meta[token];
   if (m.y <= 0) return;
+  const int most = a.shared_parts + a.own_parts;
   const int parts = parts_of(m.w, a.shared_slice, a.shared_parts) + parts_of(m.y - max(m.w, 0), a.own_slice, a.own_parts);
-  const int64_t at = (static_cast<int64_t>(token) * a.heads + head) * (a.shared_parts + a.own_parts);
-  float M = -INFINITY, L = 0.0f, O = 0.0f;
-  for (int p = 0; p < parts; ++p) M = fmaxf(M, a.part_ml[2 * (at + p)]);
-  for (int p = 0; p < parts; ++p) {
-    const float f = fast_exp2(a.part_ml[2 * (at + p)] - M);
-    L += f * a.part_ml[2 * (at + p) + 1];
-    O += f * a.part_o[(at + p) * D + d];
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * most;
+  const float4* o = reinterpret_cast<const float4*>(a.part_o) + row * most * LANES + lane;
+  float M = -INFINITY, L = 0.0f;
+  float4 O = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int p0 = 0; p0 < parts; p0 += LANES) {
+    const int n = min(LANES, parts - p0);
+    float4 v[kJoin];
+#pragma unroll
+    for (int j = 0; j < kJoin; ++j)
+      if (j < n) v[j] = o[static_cast<int64_t>(p0 + j) * LANES];
+    const float2 mine = lane < n ? ml[p0 + lane] : float2{-INFINITY, 0.0f};
+    float top = mine.x;
+#pragma unroll
+    for (int i = LANES / 2; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+    top = fmaxf(top, M);
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float f = fast_exp2(mine.x - base), keep = fast_exp2(M - base);
+    float l = f * mine.y;
+#pragma unroll
+    for (int i = LANES / 2; i > 0; i >>= 1) l += __shfl_xor(l, i);
+    L = L * keep + l;
+    M = top;
+    O = float4{O.x * keep, O.y * keep, O.z * keep, O.w * keep};
+    for (int j0 = 0; j0 < n; j0 += kJoin) {
+#pragma unroll
+      for (int j = 0; j < kJoin; ++j) {
+        if (j0 + j < n) {
+          const float w = __shfl(f, j0 + j, LANES);
+          O = float4{O.x + w * v[j].x, O.y + w * v[j].y, O.z + w * v[j].z, O.w + w * v[j].w};
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kJoin; ++j)
+        if (j0 + kJoin + j < n) v[j] = o[static_cast<int64_t>(p0 + j0 + kJoin + j) * LANES];
+    }
   }
-  a.out[m.x * a.out_stride + static_cast<int64_t>(head) * D + d] = static_cast<half_t>(O / L);
+  half_t* out = a.out + m.x * a.out_stride + static_cast<int64_t>(head) * D + 4 * lane;
+  const float inv = 1.0f / L;
+  out[0] = static_cast<half_t>(O.x * inv);
+  out[1] = static_cast<half_t>(O.y * inv);
+  out[2] = static_cast<half_t>(O.z * inv);
+  out[3] = static_cast<half_t>(O.w * inv);
+}
+
+template <int D, int DR>
+int launch(const SharedArgs& a, bool rows, int64_t wgs, hipStream_t s) {
+  const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(kThreads), 0, s, a); };
+  if constexpr (D == DR) {
+    if (rows) {
+      RH_TRY_LAUNCH(go(shared_attention_kernel<D, DR, true, true>));
+      return 0;
+    }
+  }
+  if (a.bs_shift >= 4) {
+    RH_TRY_LAUNCH(go(shared_attention_kernel<D, DR, true, false>));
+  } else {
+    RH_TRY_LAUNCH(go(shared_attention_kernel<D, DR, false, false>));
+  }
+  return 0;
 }
 
 struct Plan {
+  bool rows;
   int shared_slice, shared_parts, own_slice, own_parts, tiles, own_tiles;
 };
 
-Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_own, int heads, int kv_heads, int head_dim) {
+Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_own, int heads, int kv_heads, int head_dim,
+             int block) {
   const int group = heads / kv_heads;
-  Plan p{kStep * kWaves, 1, kStep * kWaves, 1, 1, (group + kRows - 1) / kRows};
-  const auto cut = [](int64_t wgs, int keys, int* slice, int* parts) {
+  const int64_t rows = static_cast<int64_t>(max_members) * group;
+  Plan p{};
+  // Shared tiles come in pieces of up to 16 keys of one block, straight to LDS.
+  const bool pieces = head_dim > 16 && block >= 16 && (block & (block - 1)) == 0;
+  p.rows = rows > 2 * kFew && pieces;
+  const int per = p.rows ? kWaves * kStrip : kFew;
+  p.tiles = static_cast<int>(std::max<int64_t>(1, (rows + per - 1) / per));
+  p.own_tiles = (group + kFew - 1) / kFew;
+  // As many slices as make `target` workgroups, of 128 keys at least.
+  const auto cut = [](int64_t units, int target, int keys, int* slice, int* parts) {
     const int least = kStep * kWaves;
-    const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(1, wgs));
-    *slice = std::max<int64_t>(least, ((keys + want - 1) / want + least - 1) / least * least);
+    const int64_t want = std::max<int64_t>(1, target / std::max<int64_t>(1, units));
+    *slice = static_cast<int>(std::max<int64_t>(least, ((keys + want - 1) / want + least - 1) / least * least));
     *parts = std::max(1, (keys + *slice - 1) / *slice);
   };
-  p.tiles = std::max<int64_t>(1, (static_cast<int64_t>(max_members) * group + kRows - 1) / kRows);
-  cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, max_shared, &p.shared_slice, &p.shared_parts);
-  cut(static_cast<int64_t>(n_dec) * kv_heads * p.own_tiles, max_own, &p.own_slice, &p.own_parts);
+  cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, RH_T1, max_shared, &p.shared_slice, &p.shared_parts);
+  cut(static_cast<int64_t>(n_dec) * kv_heads * p.own_tiles, RH_T2, max_own, &p.own_slice, &p.own_parts);
   return p;
 }
 
@@ -299,8 +677,12 @@ extern "C" size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_me
   if (n_dec <= 0 || n_groups < 0 || max_members < 0 || max_shared < 0 || max_own < 0 || kv_heads <= 0 || heads <= 0 ||
       heads % kv_heads || head_dim <= 0)
     return 0;
-  const Plan p = plan_of(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim);
-  return static_cast<size_t>(n_dec) * heads * (p.shared_parts + p.own_parts) * (head_dim + 2) * 4;
+  size_t parts = 0;  // enough for any block size
+  for (const int block : {1, 16}) {
+    const Plan p = plan_of(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim, block);
+    parts = std::max<size_t>(parts, p.shared_parts + p.own_parts);
+  }
+  return static_cast<size_t>(n_dec) * heads * parts * (head_dim + 2) * 4;
 }
 
 extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, const void* kpool, const void* vpool,
@@ -315,6 +697,7 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   RH_REQUIRE(head_dim == 16 || head_dim == 32 || head_dim == 64 || head_dim == 128,
              "shared prefix attention: head_dim must be 16, 32, 64 or 128");
   RH_REQUIRE(block_size > 0, "shared prefix attention: bad block size");
+  RH_REQUIRE(scale > 0.0f && scale < INFINITY, "shared prefix attention: scale must be positive");
   RH_REQUIRE(q && kpool && vpool && dec_meta && tables && out && (groups || n_groups == 0),
              "shared prefix attention: missing pointer");
   RH_REQUIRE(q_row_stride % 8 == 0 && out_row_stride >= static_cast<int64_t>(heads) * head_dim,
@@ -325,7 +708,7 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   const size_t need = rh_shared_prefix_workspace(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim);
   RH_REQUIRE(workspace_bytes >= need && (!need || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0)),
              "shared prefix attention: needs a 16-byte aligned workspace of rh_shared_prefix_workspace bytes");
-  const Plan p = plan_of(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim);
+  const Plan p = plan_of(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim, block_size);
   SharedArgs a{};
   a.q = static_cast<const half_t*>(q);
   a.q_stride = q_row_stride;
@@ -352,21 +735,31 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   a.part_ml = a.part_o + static_cast<size_t>(n_dec) * heads * (p.shared_parts + p.own_parts) * head_dim;
   a.out = static_cast<half_t*>(out);
   a.out_stride = out_row_stride;
-  const int64_t shared_wgs = static_cast<int64_t>(n_groups) * kv_heads * p.shared_parts * p.tiles;
-  const int64_t wgs = shared_wgs + static_cast<int64_t>(n_dec) * kv_heads * p.own_parts * p.own_tiles;
-  const int64_t values = static_cast<int64_t>(n_dec) * heads * head_dim;
-  RH_REQUIRE(wgs < (int64_t{1} << 31) && values < (int64_t{1} << 38), "shared prefix attention: too large");
+  const int64_t shared_units = static_cast<int64_t>(n_groups) * kv_heads * p.shared_parts;
+  const int64_t own_units = static_cast<int64_t>(n_dec) * kv_heads * p.own_parts;
+  const int64_t shared_wgs = (shared_units + 7) / 8 * 8 * p.tiles, own_wgs = (own_units + 7) / 8 * 8 * p.own_tiles;
+  const int64_t wgs = shared_wgs + own_wgs;
+  RH_REQUIRE(wgs < (int64_t{1} << 31) && static_cast<int64_t>(n_dec) * heads < (int64_t{1} << 31), "shared prefix attention: too large");
+  a.shared_units = static_cast<int>(shared_units);
+  a.own_units = static_cast<int>(own_units);
   a.shared_wgs = static_cast<int>(shared_wgs);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const auto launch = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(kThreads), 0, s, a);
+  switch (head_dim) {
+    case 16: if (int rc = launch<32, 16>(a, p.rows, wgs, s)) return rc; break;
+    case 32: if (int rc = launch<32, 32>(a, p.rows, wgs, s)) return rc; break;
+    case 64: if (int rc = launch<64, 64>(a, p.rows, wgs, s)) return rc; break;
+    default: if (int rc = launch<128, 128>(a, p.rows, wgs, s)) return rc;
+  }
+  const int64_t rows = static_cast<int64_t>(n_dec) * heads;
+  const auto join = [&](auto kernel) {
+    const int per = 1024 / head_dim;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, s, a);
   };
   switch (head_dim) {
-    case 16: RH_TRY_LAUNCH(launch(shared_attention_kernel<32, 16>)); break;
-    case 32: RH_TRY_LAUNCH(launch(shared_attention_kernel<32, 32>)); break;
-    case 64: RH_TRY_LAUNCH(launch(shared_attention_kernel<64, 64>)); break;
-    default: RH_TRY_LAUNCH(launch(shared_attention_kernel<128, 128>));
+    case 16: RH_TRY_LAUNCH(join(shared_join_kernel<16>)); break;
+    case 32: RH_TRY_LAUNCH(join(shared_join_kernel<32>)); break;
+    case 64: RH_TRY_LAUNCH(join(shared_join_kernel<64>)); break;
+    default: RH_TRY_LAUNCH(join(shared_join_kernel<128>));
   }
-  RH_TRY_LAUNCH(hipLaunchKernelGGL(shared_join_kernel, dim3(static_cast<unsigned>((values + 255) / 256)), dim3(256), 0, s, a, head_dim));
   return 0;
 }

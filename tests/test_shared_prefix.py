@@ -276,7 +276,7 @@ GOOD = dict(q=16, q_row_stride=256, kpool=16, vpool=16, dec_meta=16, groups=16, 
 @pytest.mark.parametrize("change,message", [
     ({"n_dec": -1}, "bad sizes"), ({"n_groups": -1}, "bad sizes"), ({"max_members": -1}, "bad sizes"), ({"max_own": -1}, "bad sizes"),
     ({"max_shared": -5}, "bad sizes"), ({"heads": 5}, "head counts"), ({"kv_heads": 0}, "head counts"), ({"head_dim": 48}, "head_dim"),
-    ({"block_size": 0}, "block size"), ({"q": None}, "missing pointer"), ({"groups": None}, "missing pointer"), ({"tables": None}, "missing pointer"),
+    ({"block_size": 0}, "block size"), ({"scale": 0.0}, "scale"), ({"scale": -1.0}, "scale"), ({"scale": float("nan")}, "scale"), ({"q": None}, "missing pointer"), ({"groups": None}, "missing pointer"), ({"tables": None}, "missing pointer"),
     ({"out": None}, "missing pointer"), ({"q_row_stride": 260}, "16-byte"), ({"out_row_stride": 255}, "out rows"), ({"q": 8}, "aligned"),
     ({"dec_meta": 20}, "aligned"), ({"workspace": None}, "workspace"), ({"workspace": 24}, "workspace"), ({"workspace_bytes": 64}, "workspace")])
 def test_refusals(change, message):
