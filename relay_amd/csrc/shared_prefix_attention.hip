@@ -11,7 +11,7 @@
 //   O^T[D x 32 rows] += V^T[D x 32 keys] * P^T[32 keys x 32 rows]       (MFMA 32x32x16)
 //
 // its waves taking every kWaves-th step of 32 keys, and leaves (maximum, sum, O) of the slice; the
-// slices of a row are joined by log-sum-exp in a second launch.
+// slices of a row are joined by log-sum-exp.
 #include <algorithm>
 #include <string>
 #include <type_traits>
@@ -19,10 +19,6 @@
 #include "../../include/relay_hip.h"
 #include "common.h"
 #include "lds_ring.h"
-#ifndef RH_T1
-#define RH_T1 512
-#define RH_T2 512
-#endif
 
 namespace relay_hip {
 namespace {
@@ -32,6 +28,7 @@ constexpr int kStep = 32;   // keys of a wave's step
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
 constexpr int kFew = 16;   // query rows of a workgroup whose waves take keys of their own
+constexpr int kMerge = 8;  // slices whose values are loaded at once (attend_few)
 constexpr int kRing = 4;    // 32-key tiles of K and V in LDS, where strips share them
 
 struct SharedArgs {
@@ -45,6 +42,7 @@ struct SharedArgs {
   int shared_slice, shared_parts, own_slice, own_parts, tiles, own_tiles;  // tiles: row tiles of a group, of a token
   int shared_units, shared_wgs, own_units;  // workgroups on prefixes come first
   float scale_log2;
+  int* counters;  // per token and kv head: slices that have come (zero between calls)
   float *part_o, *part_ml;
   half_t* out;
   int64_t out_stride;
@@ -53,6 +51,11 @@ struct SharedArgs {
 // Slices of `keys` keys where the launch has room for `most`; the last takes what is left.
 __device__ __forceinline__ int parts_of(int keys, int slice, int most) {
   return keys <= 0 ? 0 : min(most, (keys + slice - 1) / slice);
+}
+
+// Row tiles of kFew of some tokens (attend_few).
+__device__ __host__ __forceinline__ int64_t tiles_few(int64_t members, int group) {
+  return group <= kFew ? (members + kFew / group - 1) / (kFew / group) : members * ((group + kFew - 1) / kFew);
 }
 
 __device__ __forceinline__ float row_max(float x) {
@@ -347,7 +350,7 @@ __device__ __forceinline__ int vswz(int key) {
   return D >= 64 ? ((key >> 2) & 3) << 1 : ((key >> 2) & 1) << 1;
 }
 
-template <int D, int DR, bool SCALAR>
+template <int D, int DR, bool SCALAR, bool JOIN>
 __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* smem) {
   constexpr int CH = D / 8, KH = D / 32, DT = D / 16, VL = kStep * CH / kWave, VKEYS = kWave / CH;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -356,10 +359,17 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
   half_t* const sv = reinterpret_cast<half_t*>(smem) + w * kStep * D;
   float* const s_ml = reinterpret_cast<float*>(smem + kWaves * kFew * D * 4);  // [wave][16 rows][max, sum]
 
-  for (; sh.tile * kFew < sh.members * G; sh.tile += sh.step) {
+  // A tile has the heads of whole tokens, or up to 16 of one token's.
+  const int each = max(1, kFew / G), pieces = (G + kFew - 1) / kFew;
+  for (; sh.tile < tiles_few(sh.members, G); sh.tile += sh.step) {
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
     const int c = lane & 15, g = lane >> 4;
+    const int token0 = sh.first + sh.tile / pieces * each, head0 = sh.tile % pieces * kFew;
+    const int here = min(each, sh.first + sh.members - token0);  // tokens of the tile
+    const int rows = here * min(G - head0, kFew);
+    const auto token_of = [&](int row) { return token0 + (pieces == 1 ? row / G : 0); };
+    const auto head_of = [&](int row) { return sh.kvh * G + (pieces == 1 ? row % G : head0 + row); };
     const auto row_any = [&](int j) -> unsigned {
       j = min(j, end - 1);
       return (static_cast<unsigned>(sh.table[bshift >= 0 ? j >> bshift : j / bs]) * a.kv_heads + sh.kvh) * bs +
@@ -404,9 +414,8 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
       lookup(k0 + kWaves * kStep);
     };
 
-    const int r = sh.tile * kFew + c;
-    const bool on = r < sh.members * G;
-    const int token = sh.first + (on ? r / G : 0), head = sh.kvh * G + (on ? r % G : 0);
+    const bool on = c < rows;
+    const int token = token_of(on ? c : 0), head = head_of(on ? c : 0);
     int k0 = (SCALAR ? begin & ~15 : begin) + w * kStep;
     KvStep<D, DR> ahead[2];
     lookup(k0);
@@ -495,10 +504,9 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
       for (int e = 0; e < 4; ++e) so[(w * kFew + c) * D + ((16 * i + 4 * g + 4 * c) & (D - 1)) + e] = o[i][e];
     if (g == 0) s_ml[2 * (w * kFew + c)] = ref, s_ml[2 * (w * kFew + c) + 1] = l;
     __syncthreads();
-    const int rows = min(kFew, sh.members * G - sh.tile * kFew);
+    const int most = a.shared_parts + a.own_parts;
     for (int i = threadIdx.x; i < rows * DR; i += kThreads) {
-      const int row = i / DR, d = i % DR, rr = sh.tile * kFew + row;
-      const int tk = sh.first + rr / G, hd = sh.kvh * G + rr % G;
+      const int row = i / DR, d = i % DR;
       float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < kWaves; ++j) top = fmaxf(top, s_ml[2 * (j * kFew + row)]);
@@ -510,9 +518,67 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
         L += f * s_ml[2 * (j * kFew + row) + 1];
         O += f * so[(j * kFew + row) * D + ((d + 4 * row) & (D - 1))];
       }
-      const int64_t at = (static_cast<int64_t>(tk) * a.heads + hd) * (a.shared_parts + a.own_parts) + sh.part;
-      a.part_o[at * DR + d] = O;  // an idle token's are never read
-      if (d == 0) reinterpret_cast<float2*>(a.part_ml)[at] = float2{top, L};
+      const int64_t at = (static_cast<int64_t>(token_of(row)) * a.heads + head_of(row)) * most + sh.part;
+      if (JOIN) {
+        coherent_store(a.part_o + at * DR + d, O);
+        if (d == 0) coherent_store(a.part_ml + 2 * at, top), coherent_store(a.part_ml + 2 * at + 1, L);
+      } else {
+        a.part_o[at * DR + d] = O;  // an idle token's are never read
+        if (d == 0) reinterpret_cast<float2*>(a.part_ml)[at] = float2{top, L};
+      }
+    }
+    if constexpr (JOIN) {
+      // The last workgroup of a token's slices to come joins them. Its own stores are done before the
+      // barrier, so before it counts itself; the values travel by coherent stores and loads.
+      int* const s_last = reinterpret_cast<int*>(s_ml);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      if (static_cast<int>(threadIdx.x) < here) {
+        const int t = token0 + threadIdx.x;
+        const int4 mt = a.meta[t];
+        int last = 0;
+        if (mt.y > 0) {
+          const int of = pieces * (parts_of(mt.w, a.shared_slice, a.shared_parts) + parts_of(mt.y - max(mt.w, 0), a.own_slice, a.own_parts));
+          int* const count = a.counters + static_cast<int64_t>(t) * a.kv_heads + sh.kvh;
+          last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of - 1 ? of / pieces : 0;
+          if (last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        s_last[threadIdx.x] = last;
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < here * G * DR; i += kThreads) {
+        const int t = token0 + i / (G * DR), d = i % DR, hd = sh.kvh * G + i / DR % G;
+        const int parts = s_last[t - token0];
+        if (!parts) continue;
+        const int64_t at = (static_cast<int64_t>(t) * a.heads + hd) * most;
+        float M = -INFINITY, L = 0.0f, O = 0.0f;
+        for (int p0 = 0; p0 < parts; p0 += kMerge) {
+          float mv[kMerge], lv[kMerge], ov[kMerge], top = M;
+#pragma unroll
+          for (int j = 0; j < kMerge; ++j) {
+            if (p0 + j < parts) {
+              mv[j] = coherent_load(a.part_ml + 2 * (at + p0 + j));
+              lv[j] = coherent_load(a.part_ml + 2 * (at + p0 + j) + 1);
+              ov[j] = coherent_load(a.part_o + (at + p0 + j) * DR + d);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kMerge; ++j)
+            if (p0 + j < parts) top = fmaxf(top, mv[j]);
+          const float base = top == -INFINITY ? 0.0f : top, keep = fast_exp2(M - base);
+          L *= keep, O *= keep;
+#pragma unroll
+          for (int j = 0; j < kMerge; ++j) {
+            if (p0 + j < parts) {
+              const float f = fast_exp2(mv[j] - base);
+              L += f * lv[j];
+              O += f * ov[j];
+            }
+          }
+          M = top;
+        }
+        a.out[a.meta[t].x * a.out_stride + static_cast<int64_t>(hd) * DR + d] = static_cast<half_t>(O / L);
+      }
     }
     __syncthreads();
   }
@@ -561,65 +627,55 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D > 64
     g.end = g.part == parts - 1 ? m.y : g.begin + a.own_slice;
     g.part += parts_of(m.w, a.shared_slice, a.shared_parts);
   }
-  attend_few<D, DR, SCALAR>(a, g, smem);
+  attend_few<D, DR, SCALAR, !ROWS>(a, g, smem);
 }
 
-// Joins a row's slices: D / 4 lanes a row, four values a lane. The lanes bring 32 slices' maxima and
-// sums at once, one or two each, and kJoin slices' values at once.
-constexpr int kJoin = 8;
+// Joins a row's slices, a lane for each value. LANES slices' maxima and sums come at once, one a lane, and
+// kJoin slices' values.
+constexpr int kJoin = 16;
 template <int D>
 __global__ __launch_bounds__(256) void shared_join_kernel(const SharedArgs a) {
-  constexpr int LANES = D / 4;
-  const int lane = threadIdx.x % LANES;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+  constexpr int LANES = D < kWave ? D : kWave;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / D;
   if (row >= static_cast<int64_t>(a.n_dec) * a.heads) return;
+  const int d = static_cast<int>(i % D), lane = threadIdx.x % LANES;
   const int token = static_cast<int>(row / a.heads), head = static_cast<int>(row % a.heads);
   const int4 m = a.meta[token];
   if (m.y <= 0) return;
   const int most = a.shared_parts + a.own_parts;
   const int parts = parts_of(m.w, a.shared_slice, a.shared_parts) + parts_of(m.y - max(m.w, 0), a.own_slice, a.own_parts);
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * most;
-  const float4* o = reinterpret_cast<const float4*>(a.part_o) + row * most * LANES + lane;
-  float M = -INFINITY, L = 0.0f;
-  float4 O = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float* o = a.part_o + row * most * D + d;
+  float M = -INFINITY, L = 0.0f, O = 0.0f;
   for (int p0 = 0; p0 < parts; p0 += LANES) {
     const int n = min(LANES, parts - p0);
-    float4 v[kJoin];
+    float v[kJoin];
 #pragma unroll
     for (int j = 0; j < kJoin; ++j)
-      if (j < n) v[j] = o[static_cast<int64_t>(p0 + j) * LANES];
+      if (j < n) v[j] = o[static_cast<int64_t>(p0 + j) * D];
     const float2 mine = lane < n ? ml[p0 + lane] : float2{-INFINITY, 0.0f};
     float top = mine.x;
 #pragma unroll
-    for (int i = LANES / 2; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor(top, i));
+    for (int e = LANES / 2; e > 0; e >>= 1) top = fmaxf(top, __shfl_xor(top, e));
     top = fmaxf(top, M);
     const float base = top == -INFINITY ? 0.0f : top;
     const float f = fast_exp2(mine.x - base), keep = fast_exp2(M - base);
     float l = f * mine.y;
 #pragma unroll
-    for (int i = LANES / 2; i > 0; i >>= 1) l += __shfl_xor(l, i);
+    for (int e = LANES / 2; e > 0; e >>= 1) l += __shfl_xor(l, e);
     L = L * keep + l;
+    O *= keep;
     M = top;
-    O = float4{O.x * keep, O.y * keep, O.z * keep, O.w * keep};
     for (int j0 = 0; j0 < n; j0 += kJoin) {
 #pragma unroll
-      for (int j = 0; j < kJoin; ++j) {
-        if (j0 + j < n) {
-          const float w = __shfl(f, j0 + j, LANES);
-          O = float4{O.x + w * v[j].x, O.y + w * v[j].y, O.z + w * v[j].z, O.w + w * v[j].w};
-        }
-      }
+      for (int j = 0; j < kJoin; ++j)
+        if (j0 + j < n) O += __shfl(f, j0 + j, LANES) * v[j];
 #pragma unroll
       for (int j = 0; j < kJoin; ++j)
-        if (j0 + kJoin + j < n) v[j] = o[static_cast<int64_t>(p0 + j0 + kJoin + j) * LANES];
+        if (j0 + kJoin + j < n) v[j] = o[static_cast<int64_t>(p0 + j0 + kJoin + j) * D];
     }
   }
-  half_t* out = a.out + m.x * a.out_stride + static_cast<int64_t>(head) * D + 4 * lane;
-  const float inv = 1.0f / L;
-  out[0] = static_cast<half_t>(O.x * inv);
-  out[1] = static_cast<half_t>(O.y * inv);
-  out[2] = static_cast<half_t>(O.z * inv);
-  out[3] = static_cast<half_t>(O.w * inv);
+  a.out[m.x * a.out_stride + static_cast<int64_t>(head) * D + d] = static_cast<half_t>(O / L);
 }
 
 template <int D, int DR>
@@ -639,6 +695,9 @@ int launch(const SharedArgs& a, bool rows, int64_t wgs, hipStream_t s) {
   return 0;
 }
 
+// The counters have a fixed place at the workspace's start, so that they stay zero between calls of any shape.
+constexpr int kCounters = 65536;
+
 struct Plan {
   bool rows;
   int shared_slice, shared_parts, own_slice, own_parts, tiles, own_tiles;
@@ -652,18 +711,41 @@ Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_o
   // Shared tiles come in pieces of up to 16 keys of one block, straight to LDS.
   const bool pieces = head_dim > 16 && block >= 16 && (block & (block - 1)) == 0;
   p.rows = rows > 2 * kFew && pieces;
-  const int per = p.rows ? kWaves * kStrip : kFew;
-  p.tiles = static_cast<int>(std::max<int64_t>(1, (rows + per - 1) / per));
-  p.own_tiles = (group + kFew - 1) / kFew;
-  // As many slices as make `target` workgroups, of 128 keys at least.
-  const auto cut = [](int64_t units, int target, int keys, int* slice, int* parts) {
+  const int64_t tiles = p.rows ? (rows + kWaves * kStrip - 1) / (kWaves * kStrip) : tiles_few(max_members, group);
+  p.tiles = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), 1 << 20));
+  p.own_tiles = static_cast<int>(tiles_few(1, group));
+  // Slices of multiples of 128 keys, by what a launch of them takes (us, measured on MI355X): a start of
+  // 5, a step of 32 keys of 128 rows 1.05 at head size 128 and 0.5 below, of 128 own keys 1.5 and 0.8,
+  // in rounds of the workgroups that the card holds, and each slice's way through memory to its
+  // join. A prefix need not end before the own keys do: with 64 members on 16,384 keys and up to 1000 of
+  // their own (32/8 heads of 128) 8 / 12 / 16 / 32 slices take 79 / 69 / 72 / 86, with 45 members on 5
+  // prefixes of 1504 and up to 700 of their own 2 / 3 / 6 / 12 54 / 33 / 41 / 45.
+  const double held = 256.0 * (head_dim > 64 ? 2 : 3);
+  const double rate = 4e6;  // bytes a us
+  const auto cut = [&](int64_t units, int keys, double step, int step_keys, double part, double beside, int* slice, int* parts) {
     const int least = kStep * kWaves;
-    const int64_t want = std::max<int64_t>(1, target / std::max<int64_t>(1, units));
-    *slice = static_cast<int>(std::max<int64_t>(least, ((keys + want - 1) / want + least - 1) / least * least));
-    *parts = std::max(1, (keys + *slice - 1) / *slice);
+    double best = 0.0;
+    *slice = least, *parts = 1;
+    for (int want = 1; want <= 64; ++want) {
+      const int size = static_cast<int>((static_cast<int64_t>(keys) + static_cast<int64_t>(want) * least - 1) / (static_cast<int64_t>(want) * least)) * least;
+      if (size < least) break;
+      const int n = (keys + size - 1) / size;
+      const double rounds = static_cast<double>(units) * n / held;  // a last one is rarely full
+      const double time = (5.0 + step * size / step_keys) * (rounds <= 1.0 ? 1.0 : rounds + 0.5);
+      const double cost = std::max(time, beside) + part * n;
+      if (want == 1 || cost < best) best = cost, *slice = size, *parts = n;
+      if (size == least) break;
+    }
   };
-  cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, RH_T1, max_shared, &p.shared_slice, &p.shared_parts);
-  cut(static_cast<int64_t>(n_dec) * kv_heads * p.own_tiles, RH_T2, max_own, &p.own_slice, &p.own_parts);
+  const double own_step = head_dim > 64 ? 1.5 : 0.8;
+  // (Lengths spread below the largest: two thirds of it on average.)
+  const double own_time = 4.0 + 0.65 * n_dec * kv_heads * static_cast<double>(max_own) * head_dim * 4 / rate;
+  cut(static_cast<int64_t>(n_dec) * kv_heads * p.own_tiles, max_own, own_step, kStep * kWaves, 0.15, 0.0, &p.own_slice, &p.own_parts);
+  if (p.rows)
+    cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, max_shared, head_dim > 64 ? 1.05 : 0.5, kStep,
+        static_cast<double>(n_dec) * heads * head_dim * 8 / rate, own_time, &p.shared_slice, &p.shared_parts);
+  else
+    cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, max_shared, own_step, kStep * kWaves, 0.15, 0.0, &p.shared_slice, &p.shared_parts);
   return p;
 }
 
@@ -682,7 +764,7 @@ extern "C" size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_me
     const Plan p = plan_of(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim, block);
     parts = std::max<size_t>(parts, p.shared_parts + p.own_parts);
   }
-  return static_cast<size_t>(n_dec) * heads * parts * (head_dim + 2) * 4;
+  return kCounters * 4 + static_cast<size_t>(n_dec) * heads * parts * (head_dim + 2) * 4;
 }
 
 extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, const void* kpool, const void* vpool,
@@ -697,6 +779,7 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   RH_REQUIRE(head_dim == 16 || head_dim == 32 || head_dim == 64 || head_dim == 128,
              "shared prefix attention: head_dim must be 16, 32, 64 or 128");
   RH_REQUIRE(block_size > 0, "shared prefix attention: bad block size");
+  RH_REQUIRE(static_cast<int64_t>(n_dec) * kv_heads <= kCounters, "shared prefix attention: n_dec * kv_heads must be at most 65536");
   RH_REQUIRE(scale > 0.0f && scale < INFINITY, "shared prefix attention: scale must be positive");
   RH_REQUIRE(q && kpool && vpool && dec_meta && tables && out && (groups || n_groups == 0),
              "shared prefix attention: missing pointer");
@@ -731,7 +814,8 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   a.tiles = p.tiles;
   a.own_tiles = p.own_tiles;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.part_o = static_cast<float*>(workspace);
+  a.counters = static_cast<int*>(workspace);
+  a.part_o = static_cast<float*>(workspace) + kCounters;
   a.part_ml = a.part_o + static_cast<size_t>(n_dec) * heads * (p.shared_parts + p.own_parts) * head_dim;
   a.out = static_cast<half_t*>(out);
   a.out_stride = out_row_stride;
@@ -750,10 +834,10 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
     case 64: if (int rc = launch<64, 64>(a, p.rows, wgs, s)) return rc; break;
     default: if (int rc = launch<128, 128>(a, p.rows, wgs, s)) return rc;
   }
-  const int64_t rows = static_cast<int64_t>(n_dec) * heads;
+  if (!p.rows) return 0;
+  const int64_t values = static_cast<int64_t>(n_dec) * heads * head_dim;
   const auto join = [&](auto kernel) {
-    const int per = 1024 / head_dim;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((rows + per - 1) / per)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((values + 255) / 256)), dim3(256), 0, s, a);
   };
   switch (head_dim) {
     case 16: RH_TRY_LAUNCH(join(shared_join_kernel<16>)); break;

@@ -250,11 +250,14 @@ __global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a) {
 
 // ---- penalties, biases and masks on logits --------------------------------------------------------
 //
-// A workgroup takes kSlice consecutive logits of one row: it counts the row's history into an LDS
-// word for each of them (bit 31: in the prompt; the rest: how often in the output; integer adds, so
-// their order does not matter), notes the last bias for each, and streams its logits through once.
+// A workgroup takes a slice of consecutive logits of one row. Every logit of its slice is loaded first, 16
+// bytes a lane; while they come it counts the row's history into an LDS word for each logit (bit 31:
+// in the prompt; the rest: how often in the output; integer adds, so their order does not matter)
+// and notes the last bias for each; then one pass over the registers. Slices begin where a row's
+// address is a multiple of 16, so rows of odd vocabularies load and store 16 bytes too.
 
-constexpr int kSlice = 4096;
+constexpr int kVec = 4;                                // 16-byte loads of a thread
+constexpr int kSlice = 4 * kVec * kThreads;            // logits of a workgroup
 
 struct LogitArgs {
   const float* in;
@@ -297,60 +300,143 @@ __device__ __forceinline__ unsigned long long block_best(unsigned long long v, u
   v = waves[0];
 #pragma unroll
   for (int i = 1; i < kThreads / 64; ++i) v = waves[i] > v ? waves[i] : v;
+  __syncthreads();
   return v;
 }
 
+// BIAS: there are biases. VEC: a row's logits and results lie alike to 16 bytes.
+template <bool BIAS, bool VEC>
 __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArgs a) {
-  __shared__ unsigned s_seen[kSlice];
-  __shared__ int s_bias[kSlice];
+  __shared__ __attribute__((aligned(16))) unsigned s_seen[kSlice];
+  __shared__ __attribute__((aligned(16))) int s_bias[BIAS ? kSlice : 4];
   __shared__ unsigned long long s_best[kThreads / 64];
   __shared__ int s_last;
   const int row = blockIdx.x / a.slices, part = blockIdx.x % a.slices;
-  const int v0 = part * kSlice, n = min(kSlice, a.vocab - v0);
-  for (int i = threadIdx.x; i < kSlice; i += kThreads) s_seen[i] = 0, s_bias[i] = 0;
-  __syncthreads();
-  if (a.history) {
-    const int len = static_cast<int>(min(static_cast<int64_t>(max(a.history_len[row], 0)), a.history_stride));
-    const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
-    const int* h = a.history + row * a.history_stride;
-    for (int j = threadIdx.x; j < len; j += kThreads) {
-      const unsigned at = static_cast<unsigned>(h[j]) - static_cast<unsigned>(v0);
-      if (at < static_cast<unsigned>(n)) {
-        if (j < prompt)
-          atomicOr(&s_seen[at], 0x80000000u);
-        else
-          atomicAdd(&s_seen[at], 1u);
+  const float* in = a.in + row * a.ld;
+  float* out = a.out + row * a.out_ld;
+  // The slice's first logit; the first slice begins up to three before the row.
+  const int v0 = part * kSlice - (VEC ? static_cast<int>(reinterpret_cast<uintptr_t>(in) / 4 % 4) : 0);
+  const auto at = [&](int i) { return VEC ? 4 * (threadIdx.x + i * kThreads) : static_cast<int>(threadIdx.x) + 4 * i * kThreads; };
+  float x[kVec][4];
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int v = v0 + at(i);
+    if (VEC && v >= 0 && v + 3 < a.vocab) {
+      const float4 f = *reinterpret_cast<const float4*>(in + v);
+      x[i][0] = f.x, x[i][1] = f.y, x[i][2] = f.z, x[i][3] = f.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int u = v + (VEC ? e : e * kThreads);
+        x[i][e] = u >= 0 && u < a.vocab ? in[u] : 0.0f;
       }
     }
   }
-  const int64_t bias_at = row * a.bias_stride;
-  if (a.bias_tokens) {
-    const int len = static_cast<int>(min(static_cast<int64_t>(max(a.bias_len[row], 0)), a.bias_stride));
-    for (int j = threadIdx.x; j < len; j += kThreads) {
-      const unsigned at = static_cast<unsigned>(a.bias_tokens[bias_at + j]) - static_cast<unsigned>(v0);
-      if (at < static_cast<unsigned>(n)) atomicMax(&s_bias[at], j + 1);
-    }
-  }
-  __syncthreads();
-  const float rep = a.repetition ? a.repetition[row] : 1.0f;
-  const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
   const int mask_row = a.masks ? (a.mask_of ? a.mask_of[row] : row) : -1;
   const unsigned* mask = a.masks + (mask_row < 0 ? 0 : mask_row * a.mask_stride);
-  const float* in = a.in + row * a.ld + v0;
-  float* out = a.out + row * a.out_ld + v0;
-  unsigned long long best = 0;
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    float x = in[i];
-    if (const unsigned seen = s_seen[i]) {
-      // Each step rounded by itself, in the order of the formula.
-      x = x > 0.0f ? x / rep : mul_rounded(x, rep);
-      if (const unsigned count = seen & 0x7fffffffu) x = x - mul_rounded(freq, static_cast<float>(count)) - pres;
+  unsigned lo[kVec], hi[kVec];  // the mask's words of a thread's four logits (VEC; else read one by one)
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    lo[i] = hi[i] = ~0u;
+    const int v = v0 + at(i);
+    if (VEC && mask_row >= 0 && v < a.vocab) {
+      lo[i] = mask[max(v, 0) >> 5];
+      hi[i] = mask[min(v + 3, a.vocab - 1) >> 5];
     }
-    if (const int b = s_bias[i]) x += a.bias_values[bias_at + b - 1];
-    if (mask_row >= 0 && !((mask[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1u)) x = -INFINITY;
-    out[i] = x;
-    const unsigned long long k = token_key(x, v0 + i);
-    best = k > best ? k : best;
+  }
+  const float rep = a.repetition ? a.repetition[row] : 1.0f;
+  const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
+  const int64_t bias_at = row * a.bias_stride;
+  if (a.history || BIAS) {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      reinterpret_cast<uint4v*>(s_seen)[threadIdx.x + i * kThreads] = uint4v{0, 0, 0, 0};
+      if (BIAS) reinterpret_cast<uint4v*>(s_bias)[threadIdx.x + i * kThreads] = uint4v{0, 0, 0, 0};
+    }
+    __syncthreads();
+    const unsigned n = static_cast<unsigned>(max(0, min(kSlice, a.vocab - v0)));
+    // A token below 0 or past the vocabulary is outside every slice.
+    const auto place = [&](int token) { return token < 0 ? ~0u : static_cast<unsigned>(token) - static_cast<unsigned>(v0); };
+    if (a.history) {
+      const int len = static_cast<int>(min(static_cast<int64_t>(max(a.history_len[row], 0)), a.history_stride));
+      const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
+      const int* h = a.history + row * a.history_stride;
+      constexpr int kAhead = 8;  // tokens of a thread in flight
+      for (int j0 = threadIdx.x; j0 < len; j0 += kAhead * kThreads) {
+        int token[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) token[i] = j0 + i * kThreads < len ? h[j0 + i * kThreads] : -1;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const unsigned p = place(token[i]);
+          if (p < n) {
+            if (j0 + i * kThreads < prompt)
+              atomicOr(&s_seen[p], 0x80000000u);
+            else
+              atomicAdd(&s_seen[p], 1u);
+          }
+        }
+      }
+    }
+    if (BIAS) {
+      const int len = static_cast<int>(min(static_cast<int64_t>(max(a.bias_len[row], 0)), a.bias_stride));
+      for (int j = threadIdx.x; j < len; j += kThreads) {
+        const unsigned p = place(a.bias_tokens[bias_at + j]);
+        if (p < n) atomicMax(&s_bias[p], j + 1);
+      }
+    }
+    __syncthreads();
+  }
+  unsigned long long best = 0;
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int v = v0 + at(i);
+    unsigned seen4[4] = {0, 0, 0, 0};
+    int bias4[4] = {0, 0, 0, 0};
+    if (VEC) {
+      const uint4v s = reinterpret_cast<const uint4v*>(s_seen)[threadIdx.x + i * kThreads];
+      if (a.history) seen4[0] = s[0], seen4[1] = s[1], seen4[2] = s[2], seen4[3] = s[3];
+      if (BIAS) {
+        const uint4v b = reinterpret_cast<const uint4v*>(s_bias)[threadIdx.x + i * kThreads];
+        bias4[0] = b[0], bias4[1] = b[1], bias4[2] = b[2], bias4[3] = b[3];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (a.history) seen4[e] = s_seen[at(i) + e * kThreads];
+        if (BIAS) bias4[e] = s_bias[at(i) + e * kThreads];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int u = v + (VEC ? e : e * kThreads);
+      float y = x[i][e];
+      if (a.history) {
+        if (const unsigned seen = seen4[e]) {
+          // Each step rounded by itself, in the order of the formula.
+          y = y > 0.0f ? y / rep : mul_rounded(y, rep);
+          if (const unsigned count = seen & 0x7fffffffu) y = y - mul_rounded(freq, static_cast<float>(count)) - pres;
+        }
+      }
+      if (BIAS)
+        if (const int b = bias4[e]) y += a.bias_values[bias_at + b - 1];
+      if (u >= 0 && u < a.vocab) {
+        const unsigned word = !VEC ? (mask_row >= 0 ? mask[u >> 5] : ~0u) : u >> 5 == max(v, 0) >> 5 ? lo[i] : hi[i];
+        if (!((word >> (u & 31)) & 1u)) y = -INFINITY;
+        const unsigned long long k = token_key(y, u);
+        best = k > best ? k : best;
+      }
+      x[i][e] = y;
+    }
+    if (VEC && v >= 0 && v + 3 < a.vocab) {
+      *reinterpret_cast<float4*>(out + v) = float4{x[i][0], x[i][1], x[i][2], x[i][3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int u = v + (VEC ? e : e * kThreads);
+        if (u >= 0 && u < a.vocab) out[u] = x[i][e];
+      }
+    }
   }
   if (!a.next) return;
   best = block_best(best, s_best);
@@ -366,17 +452,17 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
   // The row's last workgroup takes the best of all slices.
   best = 0;
   for (int p = threadIdx.x; p < a.slices; p += kThreads) {
-    unsigned long long* const at = &a.best[static_cast<int64_t>(row) * a.slices + p];
-    const unsigned long long k = __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(at, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // zero again, for calls of any shape
+    unsigned long long* const from = &a.best[static_cast<int64_t>(row) * a.slices + p];
+    const unsigned long long k = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(from, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // zero again, for calls of any shape
     best = k > best ? k : best;
   }
-  __syncthreads();  // s_best is free again
   best = block_best(best, s_best);
   if (threadIdx.x == 0) a.next[row] = best ? static_cast<int>(0xffffffffu - static_cast<unsigned>(best)) : -1;
 }
 
-int slices_of(int vocab) { return (vocab + kSlice - 1) / kSlice; }
+// (A row may begin up to three logits into its first slice.)
+int slices_of(int vocab) { return static_cast<int>((static_cast<int64_t>(vocab) + 3 + kSlice - 1) / kSlice); }
 
 }  // namespace
 }  // namespace relay_hip
@@ -470,8 +556,17 @@ int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, cons
               presence, bias_tokens, bias_values, bias_stride, bias_len, masks, mask_stride, mask_of, out, out_ld, next,
               static_cast<int*>(workspace), nullptr};
   if (next) a.best = reinterpret_cast<unsigned long long*>(a.counters + (rows + 1) / 2 * 2);
-  RH_TRY_LAUNCH(hipLaunchKernelGGL(process_logits_kernel, dim3(rows * slices), dim3(kThreads), 0,
-                                   static_cast<hipStream_t>(stream), a));
+  // Every row lies alike in logits and out: equal strides, or both whole 16-byte steps.
+  const bool vec = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(out)) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(logits) % 4 == 0 && (ld - out_ld) % 4 == 0;
+  const auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, dim3(rows * slices), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+  };
+  if (bias_tokens) {
+    RH_TRY_LAUNCH(vec ? go(process_logits_kernel<true, true>) : go(process_logits_kernel<true, false>));
+  } else {
+    RH_TRY_LAUNCH(vec ? go(process_logits_kernel<false, true>) : go(process_logits_kernel<false, false>));
+  }
   return 0;
 }
 
