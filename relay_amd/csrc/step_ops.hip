@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "../../include/relay_hip.h"
 #include "common.h"
@@ -16,12 +17,18 @@ namespace {
 //
 // held = ceil(cached / B), want = ceil((cached + fresh) / B); sequence s takes want - held ids off the
 // top of the free stack, behind those of the sequences before it, and has the rows row_off[s] ..
-// row_off[s + 1] - 1. Two exclusive sums over the sequences, then one row after another by binary
-// search. One workgroup does all of it: the sums are a chain of dependent steps, and a second
-// launch costs more than the rows of a decode step.
+// row_off[s + 1] - 1: two exclusive sums over the sequences. One workgroup takes them, a sequence a
+// thread (more in several turns): they are a chain of dependent steps. Where no sequence adds more than
+// kOwnRows tokens, as in decoding, its thread writes its rows too, from what it has in registers;
+// otherwise every row finds its sequence by binary search, in a launch of its own past kOneLaunch
+// rows (48 decoding sequences 6.3 us with a search, 511 sequences of which 40 add a prompt, 26,500
+// rows, 58 us in one workgroup).
 
-constexpr int kTableThreads = 1024;
 constexpr int kSumCap = (1 << 30) - 1;  // sums stop here, past every limit that they are compared with
+constexpr int kOwnRows = 4;
+constexpr int kOneLaunch = 4096;
+constexpr int kRowThreads = 256;
+constexpr int kRowOffsets = 4096;       // row offsets that a workgroup of step_rows_kernel keeps in LDS
 
 struct StepArgs {
   const int *cached, *fresh, *shared, *group_seqs;
@@ -36,13 +43,17 @@ struct StepArgs {
 };
 
 __device__ __forceinline__ int capped_add(int a, int b) { return min(a + b, kSumCap); }
-__device__ __forceinline__ int blocks_of(int keys, int block) { return (keys + block - 1) / block; }
+__device__ __forceinline__ int blocks_of(int keys, int block) {
+  return static_cast<int>((static_cast<unsigned>(keys) + static_cast<unsigned>(block) - 1u) / static_cast<unsigned>(block));
+}
 
 struct Need {
   int rows, blocks;
 };
 
-// Inclusive sums over the workgroup and the workgroup's total.
+// Inclusive sums over the workgroup and the workgroup's total. `waves` holds an entry a wave, and is free
+// again after the caller's next barrier.
+template <int THREADS>
 __device__ Need block_scan(Need v, Need* waves, Need* total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
 #pragma unroll
@@ -53,102 +64,133 @@ __device__ Need block_scan(Need v, Need* waves, Need* total) {
   if (lane == 63) waves[w] = v;
   __syncthreads();
   Need sum = {0, 0}, before = {0, 0};
-  for (int i = 0; i < kTableThreads / 64; ++i) {
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) {
     if (i == w) before = sum;
     sum.rows = capped_add(sum.rows, waves[i].rows);
     sum.blocks = capped_add(sum.blocks, waves[i].blocks);
   }
-  __syncthreads();
   *total = sum;
   return {capped_add(before.rows, v.rows), capped_add(before.blocks, v.blocks)};
 }
 
-// Row t of the step (a row past the last is idle: no slot, an empty context).
-__device__ void fill_row(const StepArgs& a, int t, int total) {
-  if (t >= total) {
-    a.pos[t] = 0;
-    a.seq[t] = 0;
-    a.slot[t] = -1;
-    a.meta[t] = int4{t, 0, 0, 0};
-    return;
-  }
-  int lo = 0, hi = a.n_seqs;  // the last s with row_off[s] <= t that has rows
+// Row t: position p of sequence s in block `id`.
+__device__ __forceinline__ void put_row(const StepArgs& a, int t, int s, int p, int id, int shared) {
+  a.pos[t] = p;
+  a.seq[t] = s;
+  a.slot[t] = id * a.block + p % a.block;
+  a.meta[t] = int4{t, p + 1, s * a.stride, shared};
+}
+
+// A row past the step's tokens: no slot, an empty context.
+__device__ __forceinline__ void put_idle(const StepArgs& a, int t) {
+  a.pos[t] = 0;
+  a.seq[t] = 0;
+  a.slot[t] = -1;
+  a.meta[t] = int4{t, 0, 0, 0};
+}
+
+// Row t by search: its sequence is the last with row_off[s] <= t (one that has rows, as t < row_off[n_seqs]).
+__device__ __forceinline__ void find_row(const StepArgs& a, const int* row_off, int t) {
+  int lo = 0, hi = a.n_seqs;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (a.row_off[mid] <= t)
+    if (row_off[mid] <= t)
       lo = mid;
     else
       hi = mid;
   }
-  const int p = a.cached[lo] + t - a.row_off[lo];
-  const int off = lo * a.stride;
-  a.pos[t] = p;
-  a.seq[t] = lo;
-  a.slot[t] = a.tables[off + p / a.block] * a.block + p % a.block;
-  a.meta[t] = int4{t, p + 1, off, a.shared ? a.shared[lo] : 0};
+  const int p = a.cached[lo] + t - row_off[lo];
+  put_row(a, t, lo, p, a.tables[lo * a.stride + p / a.block], a.shared ? a.shared[lo] : 0);
 }
 
-__global__ __launch_bounds__(kTableThreads) void step_tables_kernel(const StepArgs a) {
-  __shared__ Need waves[kTableThreads / 64];
-  __shared__ int s_bad;
+// ROWS: the rows too.
+template <int THREADS, bool ROWS>
+__global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) {
+  __shared__ Need waves[2][THREADS / 64];
+  __shared__ int s_bad, s_most;
   const int free = *a.free_count;
-  if (threadIdx.x == 0) s_bad = 0;
-  __syncthreads();
+  if (threadIdx.x == 0) s_bad = 0, s_most = 0;
   // The sums and checks of the whole step come first: a step that does not fit changes nothing.
-  int bad = free < 0 ? RH_STEP_BAD_LENGTH : 0;
-  Need all = {0, 0};
-  for (int base = 0; base < a.n_seqs; base += kTableThreads) {
+  int bad = free < 0 ? RH_STEP_BAD_LENGTH : 0, most = 0;
+  Need all = {0, 0}, mine = {0, 0}, upto = {0, 0};  // mine, upto: of the last turn, the only one up to THREADS sequences
+  int cached = 0, shared = 0;
+  for (int base = 0, turn = 0; base < a.n_seqs; base += THREADS, turn ^= 1) {
     const int s = base + threadIdx.x;
-    Need n = {0, 0}, total;
+    mine = {0, 0};
     if (s < a.n_seqs) {
-      const int c = a.cached[s], f = a.fresh[s];
-      if (c < 0 || f < 0 || c > kSumCap || f > kSumCap - c || (a.shared && a.shared[s] < 0)) {
+      cached = a.cached[s];
+      shared = a.shared ? a.shared[s] : 0;
+      const int f = a.fresh[s];
+      if (cached < 0 || f < 0 || cached > kSumCap || f > kSumCap - cached || shared < 0) {
         bad |= RH_STEP_BAD_LENGTH;
       } else {
-        const int held = blocks_of(c, a.block), want = blocks_of(c + f, a.block);
+        const int held = blocks_of(cached, a.block), want = blocks_of(cached + f, a.block);
         if (want > a.stride) bad |= RH_STEP_TABLE_FULL;
-        n = {f, want - held};
+        mine = {f, want - held};
+        most = max(most, f);
       }
     }
-    block_scan(n, waves, &total);
+    Need total;
+    upto = block_scan<THREADS>(mine, waves[turn], &total);
     all.rows = capped_add(all.rows, total.rows);
     all.blocks = capped_add(all.blocks, total.blocks);
   }
-  for (int g = threadIdx.x; g < a.n_groups; g += kTableThreads) {
+  for (int g = threadIdx.x; g < a.n_groups; g += THREADS) {
     const int first = a.group_seqs[2 * g], count = a.group_seqs[2 * g + 1];
     if (first < 0 || count < 0 || first > a.n_seqs || count > a.n_seqs - first) bad |= RH_STEP_BAD_LENGTH;
   }
   if (all.rows > a.max_rows) bad |= RH_STEP_ROWS_FULL;
   if (all.blocks > free) bad |= RH_STEP_NO_BLOCKS;
+  if (a.n_seqs == 0) __syncthreads();  // (the scans' barriers follow s_bad's clearing)
   if (bad) atomicOr(&s_bad, bad);
+  if (most > kOwnRows) s_most = 1;
   __syncthreads();
   const int status = s_bad;
+  const bool own_rows = ROWS && !s_most;
+  if (status) all = {0, 0};
 
   Need carry = {0, 0};
-  for (int base = 0; base < a.n_seqs; base += kTableThreads) {
+  for (int base = 0, turn = 0; base < a.n_seqs; base += THREADS, turn ^= 1) {
     const int s = base + threadIdx.x;
-    Need n = {0, 0}, total;
-    int held = 0;
-    if (s < a.n_seqs && !status) {
-      const int c = a.cached[s];
-      held = blocks_of(c, a.block);
-      n = {a.fresh[s], blocks_of(c + a.fresh[s], a.block) - held};
+    if (a.n_seqs > THREADS) {
+      mine = {0, 0};
+      if (s < a.n_seqs && !status) {
+        cached = a.cached[s];
+        shared = a.shared ? a.shared[s] : 0;
+        mine = {a.fresh[s], blocks_of(cached + a.fresh[s], a.block) - blocks_of(cached, a.block)};
+      }
+      Need total;
+      upto = block_scan<THREADS>(mine, waves[turn], &total);
+      upto.rows += carry.rows, upto.blocks += carry.blocks;
+      carry.rows += total.rows, carry.blocks += total.blocks;
     }
-    const Need upto = block_scan(n, waves, &total);
+    if (status) mine = upto = {0, 0};
     if (s < a.n_seqs) {
-      const int row = carry.rows + upto.rows - n.rows, first = carry.blocks + upto.blocks - n.blocks;
+      const int row = upto.rows - mine.rows, first = upto.blocks - mine.blocks;
       a.row_off[s] = row;
-      a.last_row[s] = n.rows ? row + n.rows - 1 : 0;
+      a.last_row[s] = mine.rows ? upto.rows - 1 : 0;
       a.table_off[s] = s * a.stride;
-      for (int j = 0; j < n.blocks; ++j)
-        a.tables[static_cast<int64_t>(s) * a.stride + held + j] = a.free_blocks[free - 1 - (first + j)];
+      const int held = blocks_of(cached, a.block);
+      int* const table = a.tables + static_cast<int64_t>(s) * a.stride;
+      for (int j = 0; j < mine.blocks; ++j) table[held + j] = a.free_blocks[free - 1 - (first + j)];
+      if (own_rows) {
+        for (int j = 0; j < mine.rows; ++j) {
+          const int at = (cached + j) / a.block;
+          put_row(a, row + j, s, cached + j, at < held ? table[at] : a.free_blocks[free - 1 - (first + at - held)], shared);
+        }
+      }
     }
-    carry.rows += total.rows;
-    carry.blocks += total.blocks;
   }
-  if (threadIdx.x == 0) a.row_off[a.n_seqs] = carry.rows;
-  __syncthreads();
-  for (int g = threadIdx.x; g < a.n_groups; g += kTableThreads) {
+  if (threadIdx.x == 0) {
+    a.row_off[a.n_seqs] = all.rows;
+    a.totals[0] = all.rows;
+    a.totals[1] = all.blocks;
+    a.totals[2] = free - all.blocks;
+    a.totals[3] = status;
+  }
+  if (a.n_groups || (ROWS && !own_rows)) __syncthreads();  // row_off and the tables are read below
+  for (int g = threadIdx.x; g < a.n_groups; g += THREADS) {
     int4 v = {0, 0, 0, 0};
     if (!status) {
       const int first = a.group_seqs[2 * g], count = a.group_seqs[2 * g + 1];
@@ -158,21 +200,38 @@ __global__ __launch_bounds__(kTableThreads) void step_tables_kernel(const StepAr
     }
     a.groups[g] = v;
   }
-  for (int t = threadIdx.x; t < a.max_rows; t += kTableThreads) fill_row(a, t, carry.rows);
-  if (threadIdx.x == 0) {
-    a.totals[0] = carry.rows;
-    a.totals[1] = carry.blocks;
-    a.totals[2] = free - carry.blocks;
-    a.totals[3] = status;
+  if (ROWS) {
+    if (!own_rows)
+      for (int t = threadIdx.x; t < all.rows; t += THREADS) find_row(a, a.row_off, t);
+    for (int t = all.rows + threadIdx.x; t < a.max_rows; t += THREADS) put_idle(a, t);
   }
+}
+
+__global__ __launch_bounds__(kRowThreads) void step_rows_kernel(const StepArgs a) {
+  __shared__ int s_off[kRowOffsets];
+  const int total = a.totals[0], t = blockIdx.x * kRowThreads + threadIdx.x;
+  const bool in_lds = a.n_seqs <= kRowOffsets;
+  if (in_lds) {
+    for (int s = threadIdx.x; s < a.n_seqs; s += kRowThreads) s_off[s] = a.row_off[s];
+    __syncthreads();
+  }
+  if (t >= a.max_rows) return;
+  if (t >= total)
+    put_idle(a, t);
+  else if (in_lds)
+    find_row(a, s_off, t);
+  else
+    find_row(a, a.row_off, t);
 }
 
 // ---- norm of q and k per head, rotation, cache write --------------------------------------------
 //
 // Per head x of q and k: y = w * x / sqrt(mean(x^2) + eps), then the pair (i, i + D/2) turns by pos *
 // inv_freq[i]. A thread holds four consecutive pairs, a power of two of lanes a head, so the mean is a
-// few shuffles. The angle is taken in turns with the product in double precision: at position
-// 131,071 an fp32 product alone is off by up to 2^-8 radians, more than the fp16 results' rounding.
+// few shuffles. A wave takes HEADS sets of heads of one token, their loads together; the sines, most of
+// the arithmetic, serve all of them. The angle is taken in turns with the product in double precision:
+// at position 131,071 an fp32 product alone is off by up to 2^-8 radians, more than the fp16 results'
+// rounding.
 
 constexpr int kThreads = 256;
 
@@ -190,62 +249,81 @@ struct QkArgs {
   int heads, kv_heads, D, block;
 };
 
-template <int LANES>
-__global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a) {
-  const int t = blockIdx.x, half = a.D / 2;
-  const int h = blockIdx.y * (kThreads / LANES) + threadIdx.x / LANES, i = 4 * (threadIdx.x % LANES);
+// PLAIN: one plane and no scale, without the branches of up to 8 (2047 rows of 32/4 heads of 64 11.0 / 10.4 us).
+template <int LANES, int HEADS, bool PLAIN>
+__global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a, int sets) {
+  constexpr int PER = kWave / LANES;  // heads of a set
+  const int unit = blockIdx.x * (kThreads / kWave) + (threadIdx.x >> 6);  // (token, HEADS sets)
+  const int t = unit / sets, h0 = unit % sets * (PER * HEADS) + (threadIdx.x & 63) / LANES, i = 4 * (threadIdx.x % LANES);
+  if (t >= a.T) return;
   const int slot = a.slot[t];
+  const double p = a.pos[t];
   if (slot < 0) return;  // an idle row
-  const bool on = h < a.heads + 2 * a.kv_heads && i < half;
-  const int n = h * a.D + i;
-  const int64_t width = static_cast<int64_t>(a.heads + 2 * a.kv_heads) * a.D;
-  float x[4] = {0, 0, 0, 0}, y[4] = {0, 0, 0, 0};
-  if (on) {
-    const int64_t plane = a.T * width, e = t * width + n;
-    const float4 lo = merged4(a.qkv, a.planes, plane, e, a.scale ? a.scale + n : nullptr);
-    const float4 hi = merged4(a.qkv, a.planes, plane, e + half, a.scale ? a.scale + n + half : nullptr);
-    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
-    y[0] = hi.x, y[1] = hi.y, y[2] = hi.z, y[3] = hi.w;
-    if (a.bias) {
+  const int half = a.D / 2, total = a.heads + 2 * a.kv_heads;
+  const int64_t width = static_cast<int64_t>(total) * a.D, plane = a.T * width;
+  float x[HEADS][4], y[HEADS][4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] += a.bias[n + j], y[j] += a.bias[n + j + half];
+  for (int k = 0; k < HEADS; ++k) {
+    const int h = h0 + k * PER, n = h * a.D + i;
+    float4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+    if (PLAIN && h < total && i < half) {
+      lo = *reinterpret_cast<const float4*>(a.qkv + t * width + n);
+      hi = *reinterpret_cast<const float4*>(a.qkv + t * width + n + half);
+    } else if (h < total && i < half) {
+      lo = merged4(a.qkv, a.planes, plane, t * width + n, a.scale ? a.scale + n : nullptr);
+      hi = merged4(a.qkv, a.planes, plane, t * width + n + half, a.scale ? a.scale + n + half : nullptr);
     }
+    x[k][0] = lo.x, x[k][1] = lo.y, x[k][2] = lo.z, x[k][3] = lo.w;
+    y[k][0] = hi.x, y[k][1] = hi.y, y[k][2] = hi.z, y[k][3] = hi.w;
   }
-  const bool turned = h < a.heads + a.kv_heads;
-  float ss = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) ss += x[j] * x[j] + y[j] * y[j];
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-  if (!on) return;
-  if (turned) {
-    const float inv = 1.0f / sqrtf(ss / a.D + a.eps);
-    const float* w = h < a.heads ? a.q_norm : a.k_norm;
-    const double p = a.pos[t];
+  float sn[4] = {}, cs[4] = {};
+  if (i < half && h0 < a.heads + a.kv_heads) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float u = x[j] * inv * w[i + j], v = y[j] * inv * w[i + j + half];
       const double turns = p * (static_cast<double>(a.inv_freq[i + j]) * 0.15915494309189535);
-      float sn, cs;
-      sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-      x[j] = u * cs - v * sn;
-      y[j] = v * cs + u * sn;
+      sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sn[j], &cs[j]);
     }
   }
-  half_t* dst;
-  float f = 1.0f;
-  if (h < a.heads) {
-    dst = a.q_out + static_cast<int64_t>(t) * a.heads * a.D + n;
-    f = a.q_scale;
-  } else {
-    dst = (turned ? a.kpool : a.vpool) +
-          kv_row_offset(slot / a.block, a.kv_heads, (h - a.heads) % a.kv_heads, a.block, slot % a.block, a.D) + i;
-  }
-  half4 ox, oy;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ox[j] = static_cast<half_t>(x[j] * f), oy[j] = static_cast<half_t>(y[j] * f);
-  *reinterpret_cast<half4*>(dst) = ox;
-  *reinterpret_cast<half4*>(dst + half) = oy;
+  for (int k = 0; k < HEADS; ++k) {
+    const int h = h0 + k * PER, n = h * a.D + i;
+    const bool on = h < total && i < half;
+    if (a.bias && on) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[k][j] += a.bias[n + j], y[k][j] += a.bias[n + j + half];
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ss += x[k][j] * x[k][j] + y[k][j] * y[k][j];
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+    if (!on) continue;
+    const bool turned = h < a.heads + a.kv_heads;
+    if (turned) {
+      const float inv = 1.0f / sqrtf(ss / a.D + a.eps);
+      const float* w = h < a.heads ? a.q_norm : a.k_norm;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float u = x[k][j] * inv * w[i + j], v = y[k][j] * inv * w[i + j + half];
+        x[k][j] = u * cs[j] - v * sn[j];
+        y[k][j] = v * cs[j] + u * sn[j];
+      }
+    }
+    half_t* dst;
+    float f = 1.0f;
+    if (h < a.heads) {
+      dst = a.q_out + static_cast<int64_t>(t) * a.heads * a.D + n;
+      f = a.q_scale;
+    } else {
+      dst = (turned ? a.kpool : a.vpool) +
+            kv_row_offset(slot / a.block, a.kv_heads, (h - a.heads) % a.kv_heads, a.block, slot % a.block, a.D) + i;
+    }
+    half4 ox, oy;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) ox[j] = static_cast<half_t>(x[k][j] * f), oy[j] = static_cast<half_t>(y[k][j] * f);
+    *reinterpret_cast<half4*>(dst) = ox;
+    *reinterpret_cast<half4*>(dst + half) = oy;
+  }
 }
 
 // ---- penalties, biases and masks on logits --------------------------------------------------------
@@ -256,8 +334,8 @@ __global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a) {
 // and notes the last bias for each; then one pass over the registers. Slices begin where a row's
 // address is a multiple of 16, so rows of odd vocabularies load and store 16 bytes too.
 
-constexpr int kVec = 4;                                // 16-byte loads of a thread
-constexpr int kSlice = 4 * kVec * kThreads;            // logits of a workgroup
+// Logits of a workgroup whose threads take `vec` 16-byte loads.
+constexpr int slice_of(int vec) { return 4 * vec * kThreads; }
 
 struct LogitArgs {
   const float* in;
@@ -277,8 +355,8 @@ struct LogitArgs {
   float* out;
   int64_t out_ld;
   int* next;
-  int* counters;
-  unsigned long long* best;
+  unsigned long long* records;  // per row: a count of slices, then their best keys
+  int64_t record;               // words of a record
 };
 
 // A greater key for a greater logit, and at one logit for a lower token; 0: no logit above -inf.
@@ -305,10 +383,13 @@ __device__ __forceinline__ unsigned long long block_best(unsigned long long v, u
 }
 
 // BIAS: there are biases. VEC: a row's logits and results lie alike to 16 bytes.
-template <bool BIAS, bool VEC>
+template <bool BIAS, bool VEC, int kVec>
 __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArgs a) {
-  __shared__ __attribute__((aligned(16))) unsigned s_seen[kSlice];
-  __shared__ __attribute__((aligned(16))) int s_bias[BIAS ? kSlice : 4];
+  // A word for each logit of the slice: first what the history says, then the last bias that names it
+  // (an array of its own for these would halve the workgroups that a CU holds: 64 rows of 128,257
+  // 32 / 25 us).
+  constexpr int kSlice = slice_of(kVec);
+  __shared__ __attribute__((aligned(16))) unsigned s_word[kSlice];
   __shared__ unsigned long long s_best[kThreads / 64];
   __shared__ int s_last;
   const int row = blockIdx.x / a.slices, part = blockIdx.x % a.slices;
@@ -332,6 +413,20 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
       }
     }
   }
+  // The first tokens of the history, a round of kAhead a thread.
+  constexpr int kAhead = 8;
+  const int len = a.history ? static_cast<int>(min(static_cast<int64_t>(max(a.history_len[row], 0)), a.history_stride)) : 0;
+  const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
+  const int* h = a.history + row * a.history_stride;
+  int token[kAhead];
+  const auto tokens_from = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) token[i] = j0 + i * kThreads < len ? h[j0 + i * kThreads] : -1;
+  };
+  tokens_from(threadIdx.x);
+  const int64_t bias_at = row * a.bias_stride;
+  const int biases = BIAS ? static_cast<int>(min(static_cast<int64_t>(max(a.bias_len[row], 0)), a.bias_stride)) : 0;
+  int named = static_cast<int>(threadIdx.x) < biases ? a.bias_tokens[bias_at + threadIdx.x] : -1;
   const int mask_row = a.masks ? (a.mask_of ? a.mask_of[row] : row) : -1;
   const unsigned* mask = a.masks + (mask_row < 0 ? 0 : mask_row * a.mask_stride);
   unsigned lo[kVec], hi[kVec];  // the mask's words of a thread's four logits (VEC; else read one by one)
@@ -344,90 +439,103 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
       hi[i] = mask[min(v + 3, a.vocab - 1) >> 5];
     }
   }
-  const float rep = a.repetition ? a.repetition[row] : 1.0f;
-  const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
-  const int64_t bias_at = row * a.bias_stride;
-  if (a.history || BIAS) {
+  const auto clear = [&] {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      reinterpret_cast<uint4v*>(s_seen)[threadIdx.x + i * kThreads] = uint4v{0, 0, 0, 0};
-      if (BIAS) reinterpret_cast<uint4v*>(s_bias)[threadIdx.x + i * kThreads] = uint4v{0, 0, 0, 0};
+    for (int i = 0; i < kVec; ++i) reinterpret_cast<uint4v*>(s_word)[threadIdx.x + i * kThreads] = uint4v{0, 0, 0, 0};
+    __syncthreads();
+  };
+  // A thread's words, laid out as its logits are.
+  const auto words_of = [&](int i, unsigned (&w)[4]) {
+    if (VEC) {
+      const uint4v s = reinterpret_cast<const uint4v*>(s_word)[threadIdx.x + i * kThreads];
+      w[0] = s[0], w[1] = s[1], w[2] = s[2], w[3] = s[3];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = s_word[at(i) + e * kThreads];
+    }
+  };
+  const unsigned n = static_cast<unsigned>(max(0, min(kSlice, a.vocab - v0)));
+  // A token below 0 or past the vocabulary is outside every slice.
+  const auto place = [&](int token) { return token < 0 ? ~0u : static_cast<unsigned>(token) - static_cast<unsigned>(v0); };
+  if (len > 0) {
+    const float rep = a.repetition ? a.repetition[row] : 1.0f;
+    const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
+    clear();
+    for (int j0 = threadIdx.x; j0 < len; j0 += kAhead * kThreads) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const unsigned p = place(token[i]);
+        if (p < n) {
+          if (j0 + i * kThreads < prompt)
+            atomicOr(&s_word[p], 0x80000000u);
+          else
+            atomicAdd(&s_word[p], 1u);
+        }
+      }
+      tokens_from(j0 + kAhead * kThreads);
     }
     __syncthreads();
-    const unsigned n = static_cast<unsigned>(max(0, min(kSlice, a.vocab - v0)));
-    // A token below 0 or past the vocabulary is outside every slice.
-    const auto place = [&](int token) { return token < 0 ? ~0u : static_cast<unsigned>(token) - static_cast<unsigned>(v0); };
-    if (a.history) {
-      const int len = static_cast<int>(min(static_cast<int64_t>(max(a.history_len[row], 0)), a.history_stride));
-      const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
-      const int* h = a.history + row * a.history_stride;
-      constexpr int kAhead = 8;  // tokens of a thread in flight
-      for (int j0 = threadIdx.x; j0 < len; j0 += kAhead * kThreads) {
-        int token[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) token[i] = j0 + i * kThreads < len ? h[j0 + i * kThreads] : -1;
+    for (int i = 0; i < kVec; ++i) {
+      unsigned seen[4];
+      words_of(i, seen);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-          const unsigned p = place(token[i]);
-          if (p < n) {
-            if (j0 + i * kThreads < prompt)
-              atomicOr(&s_seen[p], 0x80000000u);
-            else
-              atomicAdd(&s_seen[p], 1u);
-          }
+      for (int e = 0; e < 4; ++e) {
+        if (seen[e]) {
+          // Each step rounded by itself, in the order of the formula.
+          float y = x[i][e];
+          y = y > 0.0f ? y / rep : mul_rounded(y, rep);
+          if (const unsigned count = seen[e] & 0x7fffffffu) y = y - mul_rounded(freq, static_cast<float>(count)) - pres;
+          x[i][e] = y;
         }
       }
     }
-    if (BIAS) {
-      const int len = static_cast<int>(min(static_cast<int64_t>(max(a.bias_len[row], 0)), a.bias_stride));
-      for (int j = threadIdx.x; j < len; j += kThreads) {
-        const unsigned p = place(a.bias_tokens[bias_at + j]);
-        if (p < n) atomicMax(&s_bias[p], j + 1);
-      }
+  }
+  if (BIAS && biases > 0) {
+    __syncthreads();  // the history's words have been read
+    clear();
+    for (int j = threadIdx.x; j < biases; j += kThreads) {
+      const unsigned p = place(named);
+      if (p < n) atomicMax(&s_word[p], static_cast<unsigned>(j + 1));
+      named = j + kThreads < biases ? a.bias_tokens[bias_at + j + kThreads] : -1;
     }
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      unsigned by[4];
+      words_of(i, by);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (by[e]) x[i][e] += a.bias_values[bias_at + by[e] - 1];
+    }
   }
   unsigned long long best = 0;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
     const int v = v0 + at(i);
-    unsigned seen4[4] = {0, 0, 0, 0};
-    int bias4[4] = {0, 0, 0, 0};
-    if (VEC) {
-      const uint4v s = reinterpret_cast<const uint4v*>(s_seen)[threadIdx.x + i * kThreads];
-      if (a.history) seen4[0] = s[0], seen4[1] = s[1], seen4[2] = s[2], seen4[3] = s[3];
-      if (BIAS) {
-        const uint4v b = reinterpret_cast<const uint4v*>(s_bias)[threadIdx.x + i * kThreads];
-        bias4[0] = b[0], bias4[1] = b[1], bias4[2] = b[2], bias4[3] = b[3];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (a.history) seen4[e] = s_seen[at(i) + e * kThreads];
-        if (BIAS) bias4[e] = s_bias[at(i) + e * kThreads];
-      }
-    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int u = v + (VEC ? e : e * kThreads);
-      float y = x[i][e];
-      if (a.history) {
-        if (const unsigned seen = seen4[e]) {
-          // Each step rounded by itself, in the order of the formula.
-          y = y > 0.0f ? y / rep : mul_rounded(y, rep);
-          if (const unsigned count = seen & 0x7fffffffu) y = y - mul_rounded(freq, static_cast<float>(count)) - pres;
-        }
-      }
-      if (BIAS)
-        if (const int b = bias4[e]) y += a.bias_values[bias_at + b - 1];
       if (u >= 0 && u < a.vocab) {
         const unsigned word = !VEC ? (mask_row >= 0 ? mask[u >> 5] : ~0u) : u >> 5 == max(v, 0) >> 5 ? lo[i] : hi[i];
-        if (!((word >> (u & 31)) & 1u)) y = -INFINITY;
-        const unsigned long long k = token_key(y, u);
+        if (!((word >> (u & 31)) & 1u)) x[i][e] = -INFINITY;
+        const unsigned long long k = token_key(x[i][e], u);
         best = k > best ? k : best;
       }
-      x[i][e] = y;
     }
+  }
+  unsigned long long* const record = a.records + row * a.record;
+  if (a.next) {
+    best = block_best(best, s_best);
+    if (threadIdx.x == 0) {
+      __hip_atomic_store(&record[1 + part], best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __builtin_amdgcn_s_waitcnt(0);
+      s_last = __hip_atomic_fetch_add(&record[0], 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.slices - 1ull;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    const int v = v0 + at(i);
     if (VEC && v >= 0 && v + 3 < a.vocab) {
       *reinterpret_cast<float4*>(out + v) = float4{x[i][0], x[i][1], x[i][2], x[i][3]};
     } else {
@@ -439,30 +547,33 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
     }
   }
   if (!a.next) return;
-  best = block_best(best, s_best);
-  if (threadIdx.x == 0) {
-    __hip_atomic_store(&a.best[static_cast<int64_t>(row) * a.slices + part], best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __builtin_amdgcn_s_waitcnt(0);
-    const int prev = __hip_atomic_fetch_add(&a.counters[row], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_last = prev == a.slices - 1;
-    if (s_last) __hip_atomic_store(&a.counters[row], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
   __syncthreads();
   if (!s_last) return;
-  // The row's last workgroup takes the best of all slices.
+  // The row's last workgroup takes the best of all slices and leaves the record zero again, for calls of any shape.
   best = 0;
-  for (int p = threadIdx.x; p < a.slices; p += kThreads) {
-    unsigned long long* const from = &a.best[static_cast<int64_t>(row) * a.slices + p];
-    const unsigned long long k = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(from, 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // zero again, for calls of any shape
-    best = k > best ? k : best;
+  for (int p = threadIdx.x; p <= a.slices; p += kThreads) {
+    const unsigned long long k = __hip_atomic_load(&record[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&record[p], 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (p) best = k > best ? k : best;
   }
   best = block_best(best, s_best);
   if (threadIdx.x == 0) a.next[row] = best ? static_cast<int>(0xffffffffu - static_cast<unsigned>(best)) : -1;
 }
 
-// (A row may begin up to three logits into its first slice.)
-int slices_of(int vocab) { return static_cast<int>((static_cast<int64_t>(vocab) + 3 + kSlice - 1) / kSlice); }
+// Slices of a row, which may begin up to three logits into its first one.
+int slices_of(int vocab, int vec) { return static_cast<int>((static_cast<int64_t>(vocab) + 3 + slice_of(vec) - 1) / slice_of(vec)); }
+
+// Small slices while they make few workgroups (each reads its row's whole history). Measured (us, histories
+// of 2000, loads 1 / 2 / 4): 1 x 32,000 7.4 / 8.3 / 10.4, 16 x 32,000 7.8 / 8.6 / 10.6, 8 x 128,256 9.6 / 9.2 /
+// 10.7, 48 x 32,000 10.5 / 10.1 / 12.3, 32 x 128,256 18.6 / 15.4 / 15.0, 64 x 128,257 41 / 30 / 30.
+int vec_of(int rows, int vocab) {
+  const int64_t wgs = static_cast<int64_t>(rows) * slices_of(vocab, 1);
+  return wgs <= 512 ? 1 : wgs <= 3000 ? 2 : 4;
+}
+
+// A row's record has 256-byte lines of its own: counts of several rows in one line are taken one after
+// another, 10 ns each (64 rows of 128,257 logits 37 us, with a line each 32).
+int64_t record_words(int vocab, int vec) { return (1 + static_cast<int64_t>(slices_of(vocab, vec)) + 31) / 32 * 32; }
 
 }  // namespace
 }  // namespace relay_hip
@@ -488,7 +599,14 @@ int rh_step_tables(const int* cached, const int* fresh, const int* shared, int n
   const StepArgs a{cached, fresh, shared, group_seqs, n_seqs, n_groups, block_size, tables, table_stride, free_blocks,
                    free_count, max_rows, row_off, last_row, table_off, pos, seq, slot,
                    reinterpret_cast<int4*>(dec_meta), reinterpret_cast<int4*>(groups), totals};
-  RH_TRY_LAUNCH(hipLaunchKernelGGL(step_tables_kernel, dim3(1), dim3(kTableThreads), 0, static_cast<hipStream_t>(stream), a));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(1), dim3(threads), 0, s, a); };
+  if (max_rows > kOneLaunch) {
+    RH_TRY_LAUNCH(n_seqs <= 256 ? go(step_tables_kernel<256, false>, 256) : go(step_tables_kernel<1024, false>, 1024));
+    RH_TRY_LAUNCH(hipLaunchKernelGGL(step_rows_kernel, dim3((max_rows + kRowThreads - 1) / kRowThreads), dim3(kRowThreads), 0, s, a));
+  } else {
+    RH_TRY_LAUNCH(n_seqs <= 256 && max_rows <= 1024 ? go(step_tables_kernel<256, true>, 256) : go(step_tables_kernel<1024, true>, 1024));
+  }
   return 0;
 }
 
@@ -509,27 +627,32 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
                  static_cast<half_t*>(vpool), static_cast<half_t*>(q_out), q_scale, heads, kv_heads, head_dim, block_size};
   const int total = heads + 2 * kv_heads;
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const auto launch = [&](auto kernel, int lanes) {
-    const int per = kThreads / lanes;
-    hipLaunchKernelGGL(kernel, dim3(T, (total + per - 1) / per), dim3(kThreads), 0, s, a);
+  const auto of_lanes = [&](auto lanes) -> int {
+    constexpr int LANES = decltype(lanes)::value;
+    const auto go = [&](auto kernel, int per_wave) -> int {
+      const int64_t sets = (total + per_wave - 1) / per_wave, wgs = (T * sets + kThreads / kWave - 1) / (kThreads / kWave);
+      RH_REQUIRE(T * sets + kThreads < (int64_t{1} << 31), "qk_norm: too many rows");
+      RH_TRY_LAUNCH(hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(kThreads), 0, s, a, static_cast<int>(sets)));
+      return 0;
+    };
+    constexpr int PER = kWave / LANES;
+    // Two sets of heads a wave once that leaves enough waves. Measured (us, one / two; bound by latency
+    // below, by memory above): 48 rows of 32/4 heads of 64 3.4 / 3.6, 256 3.7 / 3.8, 512 4.4 / 4.3, 2047 11.5 /
+    // 10.4 (floor 6.1), 4096 of 32/8 heads of 128 39 / 36 (29); three to five sets are level.
+    const bool many = static_cast<int64_t>(T) * total * LANES >= 150000;
+    if (planes == 1 && !scale) return many ? go(qk_norm_kernel<LANES, 2, true>, 2 * PER) : go(qk_norm_kernel<LANES, 1, true>, PER);
+    return many ? go(qk_norm_kernel<LANES, 2, false>, 2 * PER) : go(qk_norm_kernel<LANES, 1, false>, PER);
   };
-  if (head_dim <= 32) {
-    RH_TRY_LAUNCH(launch(qk_norm_kernel<4>, 4));
-  } else if (head_dim <= 64) {
-    RH_TRY_LAUNCH(launch(qk_norm_kernel<8>, 8));
-  } else if (head_dim <= 128) {
-    RH_TRY_LAUNCH(launch(qk_norm_kernel<16>, 16));
-  } else if (head_dim <= 256) {
-    RH_TRY_LAUNCH(launch(qk_norm_kernel<32>, 32));
-  } else {
-    RH_TRY_LAUNCH(launch(qk_norm_kernel<64>, 64));
-  }
-  return 0;
+  if (head_dim <= 32) return of_lanes(std::integral_constant<int, 4>{});
+  if (head_dim <= 64) return of_lanes(std::integral_constant<int, 8>{});
+  if (head_dim <= 128) return of_lanes(std::integral_constant<int, 16>{});
+  if (head_dim <= 256) return of_lanes(std::integral_constant<int, 32>{});
+  return of_lanes(std::integral_constant<int, 64>{});
 }
 
 size_t rh_process_logits_workspace(int rows, int vocab) {
   if (rows <= 0 || vocab <= 0) return 0;
-  return (static_cast<size_t>(rows) + 1) / 2 * 8 + static_cast<size_t>(rows) * slices_of(vocab) * 8;
+  return static_cast<size_t>(rows) * record_words(vocab, vec_of(rows, vocab)) * 8;
 }
 
 int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, const int* history, int64_t history_stride,
@@ -547,25 +670,28 @@ int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, cons
   RH_REQUIRE(!bias_tokens || (bias_values && bias_len && bias_stride >= 0 && bias_stride < kSumCap),
              "process_logits: biases need values, lengths and a stride below 2^30");
   RH_REQUIRE(!masks || mask_stride >= (static_cast<int64_t>(vocab) + 31) / 32, "process_logits: a mask row holds a bit for each token");
-  const int slices = slices_of(vocab);
+  const int loads = vec_of(rows, vocab), slices = slices_of(vocab, loads);
   RH_REQUIRE(static_cast<int64_t>(rows) * slices < (int64_t{1} << 31), "process_logits: too many rows");
   RH_REQUIRE(!next || (workspace && workspace_bytes >= rh_process_logits_workspace(rows, vocab) &&
                        reinterpret_cast<uintptr_t>(workspace) % 8 == 0),
              "process_logits: next needs an 8-byte aligned workspace of rh_process_logits_workspace bytes");
-  LogitArgs a{logits, ld, rows, vocab, slices, history, history_stride, history_len, prompt_len, repetition, frequency,
+  const LogitArgs a{logits, ld, rows, vocab, slices, history, history_stride, history_len, prompt_len, repetition, frequency,
               presence, bias_tokens, bias_values, bias_stride, bias_len, masks, mask_stride, mask_of, out, out_ld, next,
-              static_cast<int*>(workspace), nullptr};
-  if (next) a.best = reinterpret_cast<unsigned long long*>(a.counters + (rows + 1) / 2 * 2);
+              static_cast<unsigned long long*>(workspace), record_words(vocab, loads)};
   // Every row lies alike in logits and out: equal strides, or both whole 16-byte steps.
   const bool vec = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(out)) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(logits) % 4 == 0 && (ld - out_ld) % 4 == 0;
   const auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(rows * slices), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
   };
+  const auto of_loads = [&](auto bias, auto aligned) {
+    constexpr bool B = decltype(bias)::value, V = decltype(aligned)::value;
+    loads == 1 ? go(process_logits_kernel<B, V, 1>) : loads == 2 ? go(process_logits_kernel<B, V, 2>) : go(process_logits_kernel<B, V, 4>);
+  };
   if (bias_tokens) {
-    RH_TRY_LAUNCH(vec ? go(process_logits_kernel<true, true>) : go(process_logits_kernel<true, false>));
+    RH_TRY_LAUNCH(vec ? of_loads(std::true_type{}, std::true_type{}) : of_loads(std::true_type{}, std::false_type{}));
   } else {
-    RH_TRY_LAUNCH(vec ? go(process_logits_kernel<false, true>) : go(process_logits_kernel<false, false>));
+    RH_TRY_LAUNCH(vec ? of_loads(std::false_type{}, std::true_type{}) : of_loads(std::false_type{}, std::false_type{}));
   }
   return 0;
 }
