@@ -42,7 +42,8 @@ struct SharedArgs {
   int shared_slice, shared_parts, own_slice, own_parts, tiles, own_tiles;  // tiles: row tiles of a group, of a token
   int shared_units, shared_wgs, own_units;  // workgroups on prefixes come first
   float scale_log2;
-  int* counters;  // per token and kv head: slices that have come (zero between calls)
+  int* counters;  // per token and kv head, counter_step apart: slices that have come (zero between calls)
+  int counter_step;
   float *part_o, *part_ml;
   half_t* out;
   int64_t out_stride;
@@ -539,7 +540,7 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
         int last = 0;
         if (mt.y > 0) {
           const int of = pieces * (parts_of(mt.w, a.shared_slice, a.shared_parts) + parts_of(mt.y - max(mt.w, 0), a.own_slice, a.own_parts));
-          int* const count = a.counters + static_cast<int64_t>(t) * a.kv_heads + sh.kvh;
+          int* const count = a.counters + (static_cast<int64_t>(t) * a.kv_heads + sh.kvh) * a.counter_step;
           last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of - 1 ? of / pieces : 0;
           if (last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
@@ -710,7 +711,10 @@ Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_o
   Plan p{};
   // Shared tiles come in pieces of up to 16 keys of one block, straight to LDS.
   const bool pieces = head_dim > 16 && block >= 16 && (block & (block - 1)) == 0;
-  p.rows = rows > 2 * kFew && pieces;
+  // Few rows on a short prefix are joined by the last workgroup that comes, which saves a launch; a long
+  // one has more slices than one workgroup joins well. Measured (us, so / as many rows): 6 rows on 512
+  // keys 9.0 / 10.8, 8 on 4096 at head size 128 21 / 18, 16 on 16,384 48 / 31; 24 on 1024 13.6 / 11.3.
+  p.rows = pieces && (rows > kFew || max_shared > 1024);
   const int64_t tiles = p.rows ? (rows + kWaves * kStrip - 1) / (kWaves * kStrip) : tiles_few(max_members, group);
   p.tiles = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), 1 << 20));
   p.own_tiles = static_cast<int>(tiles_few(1, group));
@@ -738,14 +742,15 @@ Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_o
     }
   };
   const double own_step = head_dim > 64 ? 1.5 : 0.8;
+  const auto joined = [&](int64_t n) { return 0.09 * std::max(1.0, std::min<int64_t>(n, kFew) * head_dim / 256.0); };
   // (Lengths spread below the largest: two thirds of it on average.)
   const double own_time = 4.0 + 0.65 * n_dec * kv_heads * static_cast<double>(max_own) * head_dim * 4 / rate;
-  cut(static_cast<int64_t>(n_dec) * kv_heads * p.own_tiles, max_own, own_step, kStep * kWaves, 0.15, 0.0, &p.own_slice, &p.own_parts);
+  cut(static_cast<int64_t>(n_dec) * kv_heads * p.own_tiles, max_own, own_step, kStep * kWaves, joined(group), 0.0, &p.own_slice, &p.own_parts);
   if (p.rows)
     cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, max_shared, head_dim > 64 ? 1.05 : 0.5, kStep,
         static_cast<double>(n_dec) * heads * head_dim * 8 / rate, own_time, &p.shared_slice, &p.shared_parts);
   else
-    cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, max_shared, own_step, kStep * kWaves, 0.15, 0.0, &p.shared_slice, &p.shared_parts);
+    cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, max_shared, own_step, kStep * kWaves, joined(rows), 0.0, &p.shared_slice, &p.shared_parts);
   return p;
 }
 
@@ -815,6 +820,8 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   a.own_tiles = p.own_tiles;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.counters = static_cast<int*>(workspace);
+  // In lines of their own while there is room: counts in one line are taken one after another.
+  a.counter_step = std::min(32, kCounters / (n_dec * kv_heads));
   a.part_o = static_cast<float*>(workspace) + kCounters;
   a.part_ml = a.part_o + static_cast<size_t>(n_dec) * heads * (p.shared_parts + p.own_parts) * head_dim;
   a.out = static_cast<half_t*>(out);
