@@ -698,6 +698,7 @@ int launch(const SharedArgs& a, bool rows, int64_t wgs, hipStream_t s) {
 
 // The counters have a fixed place at the workspace's start, so that they stay zero between calls of any shape.
 constexpr int kCounters = 65536;
+constexpr int kMostKeys = 1 << 30;
 
 struct Plan {
   bool rows;
@@ -761,7 +762,7 @@ using namespace relay_hip;
 
 extern "C" size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_members, int max_shared, int max_own, int heads,
                                              int kv_heads, int head_dim) {
-  if (n_dec <= 0 || n_groups < 0 || max_members < 0 || max_shared < 0 || max_own < 0 || kv_heads <= 0 || heads <= 0 ||
+  if (n_dec <= 0 || n_groups < 0 || max_members < 0 || max_shared < 0 || max_own < 0 || max_shared > kMostKeys || max_own > kMostKeys || kv_heads <= 0 || heads <= 0 ||
       heads % kv_heads || head_dim <= 0)
     return 0;
   size_t parts = 0;  // enough for any block size
@@ -785,7 +786,8 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
              "shared prefix attention: head_dim must be 16, 32, 64 or 128");
   RH_REQUIRE(block_size > 0, "shared prefix attention: bad block size");
   RH_REQUIRE(static_cast<int64_t>(n_dec) * kv_heads <= kCounters, "shared prefix attention: n_dec * kv_heads must be at most 65536");
-  RH_REQUIRE(scale > 0.0f && scale < INFINITY, "shared prefix attention: scale must be positive");
+  RH_REQUIRE(max_shared <= kMostKeys && max_own <= kMostKeys, "shared prefix attention: at most 2^30 keys");
+  RH_REQUIRE(scale > 0.0f && scale * 1.4426950408889634f < INFINITY, "shared prefix attention: scale must be positive");
   RH_REQUIRE(q && kpool && vpool && dec_meta && tables && out && (groups || n_groups == 0),
              "shared prefix attention: missing pointer");
   RH_REQUIRE(q_row_stride % 8 == 0 && out_row_stride >= static_cast<int64_t>(heads) * head_dim,

@@ -108,7 +108,7 @@ __device__ __forceinline__ void find_row(const StepArgs& a, const int* row_off, 
 template <int THREADS, bool ROWS>
 __global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) {
   __shared__ Need waves[2][THREADS / 64];
-  __shared__ int s_bad, s_most;
+  __shared__ int s_bad, s_most, s_taken[THREADS], s_held[THREADS];
   const int free = *a.free_count;
   if (threadIdx.x == 0) s_bad = 0, s_most = 0;
   // The sums and checks of the whole step come first: a step that does not fit changes nothing.
@@ -173,13 +173,33 @@ __global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) 
       a.table_off[s] = s * a.stride;
       const int held = blocks_of(cached, a.block);
       int* const table = a.tables + static_cast<int64_t>(s) * a.stride;
-      for (int j = 0; j < mine.blocks; ++j) table[held + j] = a.free_blocks[free - 1 - (first + j)];
+      s_taken[threadIdx.x] = first;
+      s_held[threadIdx.x] = held;
+      if (!s_most)
+        for (int j = 0; j < mine.blocks; ++j) table[held + j] = a.free_blocks[free - 1 - (first + j)];
       if (own_rows) {
         for (int j = 0; j < mine.rows; ++j) {
           const int at = (cached + j) / a.block;
           put_row(a, row + j, s, cached + j, at < held ? table[at] : a.free_blocks[free - 1 - (first + at - held)], shared);
         }
       }
+    }
+    if (s_most) {
+      // Prompts take many ids: a thread an id, which finds its sequence among this turn's.
+      __syncthreads();
+      const int count = min(THREADS, a.n_seqs - base), upto_here = a.n_seqs > THREADS ? carry.blocks : all.blocks;
+      for (int k = s_taken[0] + threadIdx.x; k < upto_here; k += THREADS) {
+        int lo = 0, hi = count;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (s_taken[mid] <= k)
+            lo = mid;
+          else
+            hi = mid;
+        }
+        a.tables[static_cast<int64_t>(base + lo) * a.stride + s_held[lo] + k - s_taken[lo]] = a.free_blocks[free - 1 - k];
+      }
+      __syncthreads();
     }
   }
   if (threadIdx.x == 0) {
@@ -328,14 +348,12 @@ __global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a, int s
 
 // ---- penalties, biases and masks on logits --------------------------------------------------------
 //
-// A workgroup takes a slice of consecutive logits of one row. Every logit of its slice is loaded first, 16
-// bytes a lane; while they come it counts the row's history into an LDS word for each logit (bit 31:
-// in the prompt; the rest: how often in the output; integer adds, so their order does not matter)
-// and notes the last bias for each; then one pass over the registers. Slices begin where a row's
-// address is a multiple of 16, so rows of odd vocabularies load and store 16 bytes too.
-
-// Logits of a workgroup whose threads take `vec` 16-byte loads.
-constexpr int slice_of(int vec) { return 4 * vec * kThreads; }
+// A workgroup takes a slice of consecutive logits of one row. While they come, 16 bytes a lane, it counts
+// the row's history into an LDS word for each logit (bit 31: in the prompt; the rest: how often in the
+// output; integer adds, so their order does not matter) and notes the last bias for each; then one pass
+// over the registers. Slices begin where a row's address is a multiple of 16, so rows of odd
+// vocabularies load and store 16 bytes too. The token: each slice posts its greatest (logit, -token)
+// key, and the row's last workgroup takes the greatest of them.
 
 struct LogitArgs {
   const float* in;
@@ -387,8 +405,8 @@ template <bool BIAS, bool VEC, int kVec>
 __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArgs a) {
   // A word for each logit of the slice: first what the history says, then the last bias that names it
   // (an array of its own for these would halve the workgroups that a CU holds: 64 rows of 128,257
-  // 32 / 25 us).
-  constexpr int kSlice = slice_of(kVec);
+  // 32 / 30 us).
+  constexpr int kSlice = 4 * kVec * kThreads;
   __shared__ __attribute__((aligned(16))) unsigned s_word[kSlice];
   __shared__ unsigned long long s_best[kThreads / 64];
   __shared__ int s_last;
@@ -398,6 +416,30 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
   // The slice's first logit; the first slice begins up to three before the row.
   const int v0 = part * kSlice - (VEC ? static_cast<int>(reinterpret_cast<uintptr_t>(in) / 4 % 4) : 0);
   const auto at = [&](int i) { return VEC ? 4 * (threadIdx.x + i * kThreads) : static_cast<int>(threadIdx.x) + 4 * i * kThreads; };
+  // The first tokens of the history, kAhead pieces of four a thread (rows begin at any word), before the
+  // logits: loads return in order, and the history is worked on while the logits come.
+  constexpr int kAhead = 4;
+  struct __attribute__((packed, aligned(4))) Four {
+    int token[4];
+  };
+  const int len = a.history ? static_cast<int>(min(static_cast<int64_t>(max(a.history_len[row], 0)), a.history_stride)) : 0;
+  const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
+  const int* h = a.history + row * a.history_stride;
+  Four said[kAhead];
+  const auto tokens_from = [&](int j0) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + 4 * i * kThreads;
+      if (j - 4 * static_cast<int>(threadIdx.x) >= len) break;  // the same for all threads
+      if (j + 3 < len) {
+        said[i] = *reinterpret_cast<const Four*>(h + j);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) said[i].token[e] = j + e < len ? h[j + e] : -1;
+      }
+    }
+  };
+  tokens_from(4 * threadIdx.x);
   float x[kVec][4];
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
@@ -413,17 +455,6 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
       }
     }
   }
-  // The first tokens of the history, a round of kAhead a thread.
-  constexpr int kAhead = 8;
-  const int len = a.history ? static_cast<int>(min(static_cast<int64_t>(max(a.history_len[row], 0)), a.history_stride)) : 0;
-  const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
-  const int* h = a.history + row * a.history_stride;
-  int token[kAhead];
-  const auto tokens_from = [&](int j0) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) token[i] = j0 + i * kThreads < len ? h[j0 + i * kThreads] : -1;
-  };
-  tokens_from(threadIdx.x);
   const int64_t bias_at = row * a.bias_stride;
   const int biases = BIAS ? static_cast<int>(min(static_cast<int64_t>(max(a.bias_len[row], 0)), a.bias_stride)) : 0;
   int named = static_cast<int>(threadIdx.x) < biases ? a.bias_tokens[bias_at + threadIdx.x] : -1;
@@ -454,25 +485,31 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
       for (int e = 0; e < 4; ++e) w[e] = s_word[at(i) + e * kThreads];
     }
   };
-  const unsigned n = static_cast<unsigned>(max(0, min(kSlice, a.vocab - v0)));
-  // A token below 0 or past the vocabulary is outside every slice.
-  const auto place = [&](int token) { return token < 0 ? ~0u : static_cast<unsigned>(token) - static_cast<unsigned>(v0); };
+  // A token's place among the slice's from its first in the vocabulary on: n and more for any other token, one
+  // below 0 or past the vocabulary too.
+  const unsigned from = static_cast<unsigned>(max(v0, 0)), n = static_cast<unsigned>(max(0, min(v0 + kSlice, a.vocab) - max(v0, 0)));
+  const auto place = [&](int token) { return static_cast<unsigned>(token) - from; };
+  unsigned* const words = s_word + (max(v0, 0) - v0);
   if (len > 0) {
     const float rep = a.repetition ? a.repetition[row] : 1.0f;
     const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
     clear();
-    for (int j0 = threadIdx.x; j0 < len; j0 += kAhead * kThreads) {
+    for (int j0 = 4 * threadIdx.x; j0 - 4 * static_cast<int>(threadIdx.x) < len; j0 += 4 * kAhead * kThreads) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        const unsigned p = place(token[i]);
-        if (p < n) {
-          if (j0 + i * kThreads < prompt)
-            atomicOr(&s_word[p], 0x80000000u);
-          else
-            atomicAdd(&s_word[p], 1u);
+        if (j0 - 4 * static_cast<int>(threadIdx.x) + 4 * i * kThreads >= len) break;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const unsigned p = place(said[i].token[e]);
+          if (p < n) {
+            if (j0 + 4 * i * kThreads + e < prompt)
+              atomicOr(&words[p], 0x80000000u);
+            else
+              atomicAdd(&words[p], 1u);
+          }
         }
       }
-      tokens_from(j0 + kAhead * kThreads);
+      tokens_from(j0 + 4 * kAhead * kThreads);
     }
     __syncthreads();
 #pragma unroll
@@ -496,7 +533,7 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
     clear();
     for (int j = threadIdx.x; j < biases; j += kThreads) {
       const unsigned p = place(named);
-      if (p < n) atomicMax(&s_word[p], static_cast<unsigned>(j + 1));
+      if (p < n) atomicMax(&words[p], static_cast<unsigned>(j + 1));
       named = j + kThreads < biases ? a.bias_tokens[bias_at + j + kThreads] : -1;
     }
     __syncthreads();
@@ -560,20 +597,18 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
   if (threadIdx.x == 0) a.next[row] = best ? static_cast<int>(0xffffffffu - static_cast<unsigned>(best)) : -1;
 }
 
+// Logits of a workgroup: one 16-byte load a thread while that makes few workgroups, else two (each workgroup
+// reads its row's whole history). Measured (us, histories of 2000, one / two / four loads): 1 x 32,000
+// 7.2 / 8.0 / 10.0, 8 x 128,256 9.6 / 9.0 / 10.7, 48 x 32,000 10.5 / 9.9 / 12.3, 32 x 128,256 18.6 / 14.9 / 14.7,
+// 64 x 128,257 with 8000 41 / 27.6 / 28.6, of which reading and writing the logits take 15, the token
+// 2, the biases 3 and the history 8.
+int slice_of(int rows, int vocab) { return static_cast<int64_t>(rows) * ((vocab + 1023) / 1024) <= 512 ? 1024 : 2048; }
 // Slices of a row, which may begin up to three logits into its first one.
-int slices_of(int vocab, int vec) { return static_cast<int>((static_cast<int64_t>(vocab) + 3 + slice_of(vec) - 1) / slice_of(vec)); }
-
-// Small slices while they make few workgroups (each reads its row's whole history). Measured (us, histories
-// of 2000, loads 1 / 2 / 4): 1 x 32,000 7.4 / 8.3 / 10.4, 16 x 32,000 7.8 / 8.6 / 10.6, 8 x 128,256 9.6 / 9.2 /
-// 10.7, 48 x 32,000 10.5 / 10.1 / 12.3, 32 x 128,256 18.6 / 15.4 / 15.0, 64 x 128,257 41 / 30 / 30.
-int vec_of(int rows, int vocab) {
-  const int64_t wgs = static_cast<int64_t>(rows) * slices_of(vocab, 1);
-  return wgs <= 512 ? 1 : wgs <= 3000 ? 2 : 4;
-}
+int slices_of(int vocab, int slice) { return static_cast<int>((static_cast<int64_t>(vocab) + 3 + slice - 1) / slice); }
 
 // A row's record has 256-byte lines of its own: counts of several rows in one line are taken one after
 // another, 10 ns each (64 rows of 128,257 logits 37 us, with a line each 32).
-int64_t record_words(int vocab, int vec) { return (1 + static_cast<int64_t>(slices_of(vocab, vec)) + 31) / 32 * 32; }
+int64_t record_words(int vocab, int slice) { return (1 + static_cast<int64_t>(slices_of(vocab, slice)) + 31) / 32 * 32; }
 
 }  // namespace
 }  // namespace relay_hip
@@ -652,7 +687,7 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
 
 size_t rh_process_logits_workspace(int rows, int vocab) {
   if (rows <= 0 || vocab <= 0) return 0;
-  return static_cast<size_t>(rows) * record_words(vocab, vec_of(rows, vocab)) * 8;
+  return static_cast<size_t>(rows) * record_words(vocab, slice_of(rows, vocab)) * 8;
 }
 
 int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, const int* history, int64_t history_stride,
@@ -661,7 +696,7 @@ int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, cons
                       const int* bias_len, const uint32_t* masks, int64_t mask_stride, const int* mask_of, float* out,
                       int64_t out_ld, int* next, void* workspace, size_t workspace_bytes, void* stream) {
   if (rows == 0) return 0;
-  RH_REQUIRE(rows > 0 && vocab > 0 && ld >= vocab && out_ld >= vocab, "process_logits: bad sizes");
+  RH_REQUIRE(rows > 0 && vocab > 0 && vocab < kSumCap && ld >= vocab && out_ld >= vocab, "process_logits: bad sizes");
   RH_REQUIRE(logits && out, "process_logits: missing pointer");
   RH_REQUIRE(logits != out || ld == out_ld, "process_logits: in place needs one row stride");
   RH_REQUIRE(!history || (history_len && history_stride >= 0 && history_stride < kSumCap),
@@ -670,14 +705,14 @@ int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, cons
   RH_REQUIRE(!bias_tokens || (bias_values && bias_len && bias_stride >= 0 && bias_stride < kSumCap),
              "process_logits: biases need values, lengths and a stride below 2^30");
   RH_REQUIRE(!masks || mask_stride >= (static_cast<int64_t>(vocab) + 31) / 32, "process_logits: a mask row holds a bit for each token");
-  const int loads = vec_of(rows, vocab), slices = slices_of(vocab, loads);
+  const int slice = slice_of(rows, vocab), slices = slices_of(vocab, slice);
   RH_REQUIRE(static_cast<int64_t>(rows) * slices < (int64_t{1} << 31), "process_logits: too many rows");
   RH_REQUIRE(!next || (workspace && workspace_bytes >= rh_process_logits_workspace(rows, vocab) &&
                        reinterpret_cast<uintptr_t>(workspace) % 8 == 0),
              "process_logits: next needs an 8-byte aligned workspace of rh_process_logits_workspace bytes");
   const LogitArgs a{logits, ld, rows, vocab, slices, history, history_stride, history_len, prompt_len, repetition, frequency,
               presence, bias_tokens, bias_values, bias_stride, bias_len, masks, mask_stride, mask_of, out, out_ld, next,
-              static_cast<unsigned long long*>(workspace), record_words(vocab, loads)};
+              static_cast<unsigned long long*>(workspace), record_words(vocab, slice)};
   // Every row lies alike in logits and out: equal strides, or both whole 16-byte steps.
   const bool vec = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(out)) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(logits) % 4 == 0 && (ld - out_ld) % 4 == 0;
@@ -686,7 +721,7 @@ int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, cons
   };
   const auto of_loads = [&](auto bias, auto aligned) {
     constexpr bool B = decltype(bias)::value, V = decltype(aligned)::value;
-    loads == 1 ? go(process_logits_kernel<B, V, 1>) : loads == 2 ? go(process_logits_kernel<B, V, 2>) : go(process_logits_kernel<B, V, 4>);
+slice == 1024 ? go(process_logits_kernel<B, V, 1>) : go(process_logits_kernel<B, V, 2>);
   };
   if (bias_tokens) {
     RH_TRY_LAUNCH(vec ? of_loads(std::true_type{}, std::true_type{}) : of_loads(std::true_type{}, std::false_type{}));
