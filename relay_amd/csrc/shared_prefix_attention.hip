@@ -75,47 +75,35 @@ __device__ __forceinline__ int kswz(int key) {
 template <int D>
 struct Strip {
   float16v o[D / 32];
-  float ref, l;    // the row's offset in the log2 domain (-inf: no key seen), this lane's share of its sum
-  bool have_ref;   // wave-uniform: every row has one
+  float ref, l;  // the row's maximum in the log2 domain (-inf: no key seen), this lane's share of its sum
 };
 
-// P = exp2(S scale - ref), the sum and the offset. An offset moves only when a row's weights pass 2^15
-// (a lane's sum tells): O and l are rescaled on a few steps, not on all (64 multiplies a step at
-// head size 128). A masked key's S is -inf.
+// P = exp2(S scale - ref) with the row's running maximum as ref, and the sum. O and l are rescaled where a
+// row of the wave has a new maximum: on fewer and fewer steps. (An offset that moved only before a
+// weight could overflow fp16 took up to 5% less time, and doubled the noise of the weights' rounding:
+// with a maximum as offset the greatest weight, which counts most, is exactly 1.) A masked key's S is -inf.
 template <int D>
 __device__ __forceinline__ void weigh(Strip<D>& st, const float16v& s, half8 (&p)[2], float scale) {
-  float sum = 0.0f;
-  const auto weights = [&](float nref) {
-    sum = 0.0f;
+  float mx = s[0];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float x = fast_exp2(fmaf(s[e], scale, nref));
-      sum += x;
-      p[e >> 3][e & 7] = static_cast<half_t>(x);
-    }
-  };
-  bool slow = !st.have_ref;
-  if (!slow) {
-    weights(-st.ref);
-    slow = __ballot(!(sum <= 32768.0f)) != 0;
-  }
-  if (slow) {
-    float mx = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[e] * scale);
-    mx = row_max(mx);
-    float alpha = 1.0f;
-    if (mx > st.ref + 8.0f || st.ref == -INFINITY) {
-      alpha = st.ref == -INFINITY ? 0.0f : fast_exp2(st.ref - mx);
-      st.ref = mx;
-    }
-    weights(st.ref == -INFINITY ? 0.0f : -st.ref);
+  for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+  mx = row_max(mx) * scale;
+  if (__ballot(mx > st.ref) != 0) {
+    const float ref = fmaxf(mx, st.ref), alpha = ref == -INFINITY ? 1.0f : fast_exp2(st.ref - ref);
+    st.ref = ref;
     st.l *= alpha;
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
       for (int e = 0; e < 16; ++e) st.o[i][e] *= alpha;
-    st.have_ref = __ballot(st.ref == -INFINITY) == 0;
+  }
+  const float nref = st.ref == -INFINITY ? 0.0f : -st.ref;
+  float sum = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const float x = fast_exp2(fmaf(s[e], scale, nref));
+    sum += x;
+    p[e >> 3][e & 7] = static_cast<half_t>(x);
   }
   st.l += sum;
 }
@@ -257,7 +245,7 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
 #pragma unroll
     for (int i = 0; i < MK; ++i) asm volatile("" : "+v"(qb[i]));  // q is here: the loop waits for its own loads alone
     Strip<D> st;
-    st.ref = -INFINITY, st.l = 0.0f, st.have_ref = false;
+    st.ref = -INFINITY, st.l = 0.0f;
 #pragma unroll
     for (int i = 0; i < DT; ++i)
 #pragma unroll
