@@ -537,7 +537,8 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
  *                        right and the call gets slower
  *  workspace             rh_shared_prefix_workspace bytes for the same arguments, 16-byte aligned, all
  *                        zero before its first call (each call leaves what the next needs)
- * q, pools, tables, scale, out, head sizes and block sizes as for rh_paged_decode_attention. */
+ * q, pools, tables, out, head sizes and block sizes as for rh_paged_decode_attention; scale positive;
+ * n_dec * kv_heads at most 65536. */
 int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, const void* kpool, const void* vpool,
                                const int* dec_meta, const int* groups, const int* tables, int n_dec, int n_groups,
                                int max_members, int max_shared, int max_own, int heads, int kv_heads, int head_dim,
@@ -546,13 +547,24 @@ int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, const void* 
 size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_members, int max_shared, int max_own, int heads,
                                   int kv_heads, int head_dim);
 
+/* Host-side: which tokens of a step share a prefix. tokens [n_dec][4] are rh_paged_decode_attention's
+ * descriptors (row, context, table offset, unused) and tables their block tables, both in host
+ * memory. Writes the descriptors in the order of their groups, with their shared keys, to dec_meta
+ * [n_dec][4], the groups to groups (room for n_dec [4]) and the largest group, the most shared keys and the
+ * most keys behind them to limits [3]: max_members, max_shared, max_own of the attention. A group's
+ * shared keys are whole blocks that all its members' tables begin with and their contexts hold, at
+ * least min_shared keys; groups are chosen to save the most reads. Returns their number or a
+ * negative error code. Quadratic in the tokens of one prefix. */
+int rh_shared_prefix_groups(const int* tokens, const int* tables, int n_dec, int block_size, int min_shared,
+                            int* dec_meta, int* groups, int* limits);
+
 /* Penalties, biases and grammar masks on logits, and the greedy token of each row. For token v of
  * row r, each step rounded to fp32:
  *   seen in the row's history:        x = x > 0 ? x / repetition[r] : x * repetition[r]
  *   count > 0 times in its output:    x = x - frequency[r] * count - presence[r]
  *   named by its biases:              x = x + value (the last one, if several name it)
  *   not allowed by its mask:          x = -inf
- *  logits [rows] rows ld apart, out [rows] rows out_ld apart; out may be logits (with one ld)
+ *  logits, out           rows ld and out_ld apart; out may be logits (with one ld), else they lie apart
  *  history               row r: the first history_len[r] tokens at history + r * history_stride, of
  *                        which the first prompt_len[r] (NULL: none) are the prompt and the rest the
  *                        output; NULL: no penalties. Tokens outside 0 .. vocab - 1 count for nothing
@@ -566,7 +578,7 @@ size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_members, int 
  *  workspace             only for next: rh_process_logits_workspace bytes, 8-byte aligned, all zero before
  *                        its first call; each call leaves it all zero, so calls of other sizes
  *                        may share it
- * Lengths are taken as 0 below 0 and as the stride above it. */
+ * Lengths are taken as 0 below 0 and as the stride above it. vocab below 2^30 - 1. */
 int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, const int* history, int64_t history_stride,
                       const int* history_len, const int* prompt_len, const float* repetition, const float* frequency,
                       const float* presence, const int* bias_tokens, const float* bias_values, int64_t bias_stride,

@@ -3,18 +3,27 @@
 // shared prefix are read once for all members of a group and not once for each.
 //
 // Per kv head the members' query heads form one matrix of members * G rows against the prefix's K
-// and V; the keys behind the prefix are each token's own. Both are the same work on another
-// list of rows and range of keys: a workgroup takes 32 rows and a slice of keys,
+// and V; the keys behind the prefix are each token's own. A workgroup of four waves takes some rows
+// and a slice of keys, and leaves (maximum, sum, O) of each row; a row's slices are joined by
+// log-sum-exp. Softmax in the log2 domain, sums, maxima and O in fp32; the weights are rounded to fp16
+// for the product with V, as in the other attention kernels: an MFMA operand of twice the width
+// would double that product. Two ways through a slice:
 //
-//   S^T[32 keys x 32 rows] = K[32 keys x D] * Q^T[D x 32 rows]          (MFMA 32x32x16)
-//   online softmax per row in the log2 domain, in fp32 (lanes c and c + 32 hold row c)
-//   O^T[D x 32 rows] += V^T[D x 32 keys] * P^T[32 keys x 32 rows]       (MFMA 32x32x16)
+//  - many rows (prefixes of more than 16 rows or 1024 keys): 128 rows, 32 a wave, on tiles of K and V that
+//    the waves share in LDS (attend_rows). Bound by the chain of a step (LDS reads, products, weights:
+//    no one of them taken out made it faster by over a tenth) and by K and V from memory.
+//  - few rows (own keys, short prefixes): 16 rows, the waves on keys of their own, K straight into MFMA
+//    operands (attend_few). Bound by memory: 64 x 1000 own keys, 8 kv heads of 128 (ragged, 164 MB) 40 us.
 //
-// its waves taking every kWaves-th step of 32 keys, and leaves (maximum, sum, O) of the slice; the
-// slices of a row are joined by log-sum-exp.
+// One launch does both, prefixes first: the prefix's products run beside the own keys' loads. 64 members on
+// 16,384 keys with up to 1000 of their own (231 MB, 18 GFLOP) take 61 us, the join 7. Prefix and own keys in
+// workgroups of eight waves, one a CU, or staged through registers, whose reloads from scratch waited
+// for every load in flight, took 107.
 #include <algorithm>
+#include <exception>
 #include <string>
 #include <type_traits>
+#include <vector>
 
 #include "../../include/relay_hip.h"
 #include "common.h"
@@ -747,6 +756,67 @@ Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_o
 }  // namespace relay_hip
 
 using namespace relay_hip;
+
+extern "C" int rh_shared_prefix_groups(const int* tokens, const int* tables, int n_dec, int block_size, int min_shared,
+                                       int* dec_meta, int* groups, int* limits) {
+  RH_REQUIRE(n_dec >= 0 && block_size > 0 && min_shared >= 0, "shared prefix groups: bad sizes");
+  RH_REQUIRE(limits && (n_dec == 0 || (tokens && tables && dec_meta && groups)), "shared prefix groups: missing pointer");
+  limits[0] = limits[1] = limits[2] = 0;
+  try {
+    // Tokens in the order of their tables' whole blocks; neighbours then share the most.
+    std::vector<int> order(n_dec);
+    for (int i = 0; i < n_dec; ++i) order[i] = i;
+    const auto blocks = [&](int i) { return std::max(0, tokens[4 * i + 1]) / block_size; };
+    const auto table = [&](int i) { return tables + tokens[4 * i + 2]; };
+    std::stable_sort(order.begin(), order.end(), [&](int x, int y) {
+      return std::lexicographical_compare(table(x), table(x) + blocks(x), table(y), table(y) + blocks(y));
+    });
+    std::vector<int> alike(n_dec, 0);  // whole blocks that a token shares with the one before it
+    for (int i = 1; i < n_dec; ++i) {
+      const int n = std::min(blocks(order[i - 1]), blocks(order[i]));
+      alike[i] = static_cast<int>(std::mismatch(table(order[i]), table(order[i]) + n, table(order[i - 1])).first - table(order[i]));
+    }
+    // Runs of neighbours that save the most reads, (members - 1) * shared blocks each.
+    std::vector<int64_t> saved(n_dec + 1, 0);
+    std::vector<int> from(n_dec + 1, 0);
+    const int least = std::max(1, (min_shared + block_size - 1) / block_size);
+    for (int end = 1; end <= n_dec; ++end) {
+      saved[end] = saved[end - 1];
+      from[end] = end - 1;
+      int common = INT32_MAX;
+      for (int first = end - 2; first >= 0; --first) {
+        common = std::min(common, alike[first + 1]);
+        if (common < least) break;
+        const int64_t with = saved[first] + static_cast<int64_t>(end - first - 1) * common;
+        if (with > saved[end]) saved[end] = with, from[end] = first;
+      }
+    }
+    std::vector<int> ends;
+    for (int end = n_dec; end > 0; end = from[end]) ends.push_back(end);
+    int n_groups = 0;
+    for (std::size_t e = ends.size(); e-- > 0;) {
+      const int end = ends[e], first = from[end], members = end - first;
+      int common = members > 1 ? INT32_MAX : 0;
+      for (int i = first + 1; i < end; ++i) common = std::min(common, alike[i]);
+      const int shared = common * block_size;
+      for (int i = first; i < end; ++i) {
+        const int* t = tokens + 4 * order[i];
+        const int meta[4] = {t[0], t[1], t[2], shared};
+        std::copy(meta, meta + 4, dec_meta + 4 * i);
+        limits[2] = std::max(limits[2], t[1] - shared);
+      }
+      if (members == 1) continue;
+      const int record[4] = {first, members, shared, tokens[4 * order[first] + 2]};
+      std::copy(record, record + 4, groups + 4 * n_groups++);
+      limits[0] = std::max(limits[0], members);
+      limits[1] = std::max(limits[1], shared);
+    }
+    return n_groups;
+  } catch (const std::exception& e) {
+    set_error(std::string("shared prefix groups: ") + e.what());
+    return -1;
+  }
+}
 
 extern "C" size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_members, int max_shared, int max_own, int heads,
                                              int kv_heads, int head_dim) {

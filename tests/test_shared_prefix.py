@@ -267,6 +267,90 @@ def test_graph_replays_and_streams(torch_mod, dev):
         torch.cuda.synchronize()
 
 
+# ---- groups of a step, found on the host ---------------------------------------------------------------
+
+def groups_of(tokens, tables, bs, least):
+    t, tab = np.ascontiguousarray(tokens, np.int32), np.ascontiguousarray(tables, np.int32)
+    n = len(t)
+    meta, groups, limits = np.full((n, 4), -9, np.int32), np.full((n, 4), -9, np.int32), np.full(3, -9, np.int32)
+    got = _lib.lib().rh_shared_prefix_groups(t.ctypes.data, tab.ctypes.data, n, bs, least, meta.ctypes.data, groups.ctypes.data, limits.ctypes.data)
+    assert got >= 0, _lib.last_error()
+    assert (groups[got:] == -9).all()
+    return meta, groups[:got], limits
+
+
+def saved_at_most(rows, ctx, bs, least):
+    """The most blocks that any partition into groups saves, by trying all of them."""
+    def partitions(items):
+        if not items:
+            yield []
+            return
+        for rest in partitions(items[1:]):
+            yield [[items[0]]] + rest
+            for k in range(len(rest)):
+                yield rest[:k] + [[items[0]] + rest[k]] + rest[k + 1:]
+
+    def common(group):
+        n = min(ctx[i] // bs for i in group)
+        k = 0
+        while k < n and len({rows[i][k] for i in group}) == 1:
+            k += 1
+        return k if k * bs >= max(least, 1) else 0
+    return max(sum((len(g) - 1) * common(g) for g in p) for p in partitions(list(range(len(rows)))))
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_groups_save_the_most_and_share_what_they_say(seed):
+    r = np.random.default_rng(seed)
+    bs, n, least = int(r.choice([1, 4, 16])), int(r.integers(1, 8)), int(r.choice([0, 5, 33]))
+    prompts = [list(r.integers(0, 3, 6)) for _ in range(2)]
+    rows, ctx, tables, tokens = [], [], [], []
+    for i in range(n):
+        own = [int(x) for x in r.integers(0, 3, 7)]
+        cut = int(r.integers(0, 7))
+        rows.append([int(x) for x in prompts[int(r.integers(0, 2))][:cut]] + own[cut:])
+        ctx.append(int(r.integers(0, 7 * bs + 1)))
+        tokens.append([10 + i, ctx[i], len(tables), 77])
+        tables += rows[i]
+    meta, groups, limits = groups_of(tokens, tables, bs, least)
+    assert sorted(meta[:, 0]) == [10 + i for i in range(n)]
+    grouped = np.zeros(n, bool)
+    for first, members, shared, off in groups:
+        assert members > 1 and shared % bs == 0 and shared >= max(1, least)
+        grouped[first:first + members] = True
+        for t in meta[first:first + members]:
+            i = t[0] - 10
+            assert t[3] == shared and t[1] == ctx[i] >= shared and t[2] == tokens[i][2]
+            assert tables[off:off + shared // bs] == rows[i][:shared // bs]
+    assert (meta[~grouped, 3] == 0).all()
+    assert sum((m - 1) * s for _, m, s, _ in groups) == saved_at_most(rows, ctx, bs, least) * bs
+    assert limits.tolist() == [max([g[1] for g in groups], default=0), max([g[2] for g in groups], default=0), max(0, *(meta[:, 1] - meta[:, 3]))]
+
+
+def test_groups_of_nothing_and_refusals():
+    lib = _lib.lib()
+    lim = np.zeros(3, np.int32)
+    assert lib.rh_shared_prefix_groups(None, None, 0, 16, 0, None, None, lim.ctypes.data) == 0
+    for args in ((None, None, -1, 16, 0, None, None, lim.ctypes.data), (None, None, 0, 0, 0, None, None, lim.ctypes.data),
+                 (None, None, 0, 16, -1, None, None, lim.ctypes.data), (None, None, 3, 16, 0, None, None, lim.ctypes.data), (None, None, 0, 16, 0, None, None, None)):
+        assert lib.rh_shared_prefix_groups(*args) < 0 and "shared prefix groups" in _lib.last_error()
+
+
+@gpu
+def test_groups_from_the_host_give_the_decode_kernels_attention(torch_mod, dev):
+    """Ungrouped descriptors through rh_shared_prefix_groups: the same attention as without sharing."""
+    case = Case([(5, 320), (1, 0), (4, 96), (2, 16)], [33, 150, 7], 32, 4, 64, seed=13)
+    tokens = [[m[0], m[1], m[2], 0] for m in np.random.default_rng(1).permutation(case.meta).tolist()]
+    meta, groups, limits = groups_of(tokens, case.tables, case.bs, 32)
+    assert sorted((g[1], g[2]) for g in groups) == [(4, 96), (5, 320)]
+    case.meta, case.groups = meta.tolist(), groups.tolist()
+    want, tol = Case([(5, 320), (1, 0), (4, 96), (2, 16)], [33, 150, 7], 32, 4, 64, seed=13).oracle()
+    call = Call(torch_mod, dev, case, hints=tuple(int(x) for x in limits))
+    call()
+    torch_mod.cuda.synchronize()
+    assert (np.abs(call.out.double().cpu().numpy() - want) <= tol).all()
+
+
 # ---- refusals (nothing is launched: the CPU suffices) ------------------------------------------------
 
 GOOD = dict(q=16, q_row_stride=256, kpool=16, vpool=16, dec_meta=16, groups=16, tables=16, n_dec=4, n_groups=1, max_members=4, max_shared=64, max_own=16,
@@ -278,7 +362,8 @@ GOOD = dict(q=16, q_row_stride=256, kpool=16, vpool=16, dec_meta=16, groups=16, 
     ({"max_shared": -5}, "bad sizes"), ({"heads": 5}, "head counts"), ({"kv_heads": 0}, "head counts"), ({"head_dim": 48}, "head_dim"),
     ({"block_size": 0}, "block size"), ({"scale": 0.0}, "scale"), ({"scale": -1.0}, "scale"), ({"scale": float("nan")}, "scale"), ({"q": None}, "missing pointer"), ({"groups": None}, "missing pointer"), ({"tables": None}, "missing pointer"),
     ({"out": None}, "missing pointer"), ({"q_row_stride": 260}, "16-byte"), ({"out_row_stride": 255}, "out rows"), ({"q": 8}, "aligned"),
-    ({"dec_meta": 20}, "aligned"), ({"workspace": None}, "workspace"), ({"workspace": 24}, "workspace"), ({"workspace_bytes": 64}, "workspace")])
+    ({"dec_meta": 20}, "aligned"), ({"workspace": None}, "workspace"), ({"workspace": 24}, "workspace"), ({"workspace_bytes": 64}, "workspace"),
+    ({"max_shared": (1 << 30) + 1}, "2^30"), ({"max_own": (1 << 31) - 1}, "2^30"), ({"n_dec": 40000}, "65536"), ({"scale": 3e38}, "scale")])
 def test_refusals(change, message):
     lib = _lib.lib()
     assert lib.rh_shared_prefix_attention(*{**GOOD, **change}.values()) != 0

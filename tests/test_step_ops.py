@@ -524,7 +524,7 @@ LOGITS = dict(logits=16, ld=100, rows=2, vocab=100, history=16, history_stride=8
 
 
 @pytest.mark.parametrize("change,message", [
-    ({"rows": -1}, "bad sizes"), ({"vocab": 0}, "bad sizes"), ({"ld": 99}, "bad sizes"), ({"out_ld": 99}, "bad sizes"), ({"logits": None}, "missing"),
+    ({"rows": -1}, "bad sizes"), ({"vocab": 0}, "bad sizes"), ({"vocab": 1 << 30, "ld": 1 << 30, "out_ld": 1 << 30}, "bad sizes"), ({"ld": 99}, "bad sizes"), ({"out_ld": 99}, "bad sizes"), ({"logits": None}, "missing"),
     ({"out": None}, "missing"), ({"out": 16, "out_ld": 101}, "in place"), ({"history_len": None}, "lengths"), ({"history_stride": -1}, "stride"),
     ({"history": None}, "need a history"), ({"bias_tokens": 16}, "biases need"), ({"bias_tokens": 16, "bias_values": 16, "bias_len": 16, "bias_stride": -1}, "biases need"),
     ({"masks": 16, "mask_stride": 3}, "a bit for each"), ({"workspace": None}, "workspace"), ({"workspace": 20}, "workspace"), ({"workspace_bytes": 8}, "workspace"),
