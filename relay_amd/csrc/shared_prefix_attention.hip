@@ -212,22 +212,27 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
     int entry;
     const auto first16 = [&](int j) { return min(g.begin + j * kStep + 16 * (w & 1), (g.end - 1) & ~15); };
     const auto lookup = [&](int j) { entry = entries[first16(j) >> sh]; };
-    const auto send = [&](int j) {
-      const int key = first16(j);
-      const half_t* const base = pool + ((static_cast<int64_t>(entry) * a.kv_heads + g.kvh) * bs + (key & (bs - 1))) * D;
-      const int last = g.end - 1 - key;
+    uint32_t piece[PER16];  // a lane's offsets in 16 keys
+    const auto pieces_to = [&](int last) {
 #pragma unroll
       for (int i = 0; i < PER16; ++i) {
-        const int at = i * KEYS + lane / CH, k = 16 * (w & 1) + at;  // of the 16 keys, of the tile
-        const int cc = (lane % CH) ^ kswz<D>(k);
-        global_to_lds(base, (min(at, last) * D + 8 * cc) * 2,  // past the end: the last key again
-                      lds + (j % kRing * 2 * TILE + (w >> 1) * TILE + (16 * (w & 1) + i * KEYS) * D) * 2);
+        const int at = i * KEYS + lane / CH;
+        piece[i] = (min(at, last) * D + 8 * ((lane % CH) ^ kswz<D>(16 * (w & 1) + at))) * 2;
       }
+    };
+    pieces_to(15);
+    const auto send = [&](int j, int slot) {
+      const int key = first16(j);
+      const half_t* const base = pool + ((static_cast<int64_t>(entry) * a.kv_heads + g.kvh) * bs + (key & (bs - 1))) * D;
+      if (g.end - key < 16) pieces_to(g.end - 1 - key);  // the last tile: past the end the last key again
+#pragma unroll
+      for (int i = 0; i < PER16; ++i)
+        global_to_lds(base, piece[i], lds + (slot * 2 * TILE + (w >> 1) * TILE + (16 * (w & 1) + i * KEYS) * D) * 2);
     };
     lookup(0);
     for (int j = 0; j < kRing - 1; ++j)
       if (j < n) {
-        send(j);
+        send(j, j);
         lookup(j + 1);
       }
 
@@ -263,10 +268,10 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
     // Step j has S of tile j. It waits for tile j + 1 (one barrier, which also frees tile j - 1's
     // buffer to be sent for again), reads its K while tile j's weights are computed, and tile j's V
     // while the next S is: the LDS reads' latency lies under other work.
-    const auto tile_at = [&](int j) { return ring + j % kRing * 2 * TILE; };
+    // (Unrolled by the ring, so that a buffer's address is a constant beside the lane's.)
     half8 k[MK];
-    const auto read_k = [&](int j) {
-      const half_t* const kt = tile_at(j) + c * D;
+    const auto read_k = [&](int slot) {
+      const half_t* const kt = ring + slot * 2 * TILE + c * D;
 #pragma unroll
       for (int i = 0; i < MK; ++i) k[i] = *reinterpret_cast<const half8*>(kt + (((2 * i + hh) ^ kswz<D>(c)) << 3));
     };
@@ -282,25 +287,33 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
     const bool busy = (g.tile * kWaves + w) * kStrip < g.members * G;  // a wave without rows only brings tiles
     read_k(0);
     scores();
-    for (int j = 0; j < n; ++j) {
+    const auto step = [&](int j, auto slot_tag) {
+      constexpr int SLOT = decltype(slot_tag)::value;
       const bool more = j + 1 < n;
       if (more) wait_stages<PER16, kRing - 3>(min(n - 2 - j, kRing - 3));
       ring_barrier();
       if (j + kRing - 1 < n) {
-        send(j + kRing - 1);
+        send(j + kRing - 1, (SLOT + kRing - 1) % kRing);
         lookup(j + kRing);
       }
-      if (!busy) continue;
-      if (more) read_k(j + 1);
+      if (!busy) return;
+      if (more) read_k((SLOT + 1) % kRing);
       __builtin_amdgcn_sched_barrier(0);
       const int k0 = g.begin + j * kStep;
       if (k0 + kStep > all) mask_keys(s, k0, g.begin, lim);
       half8 p[2], v[2][DT];
       weigh(st, s, p, a.scale_log2);
-      read_v<D>(v, tile_at(j) + TILE);
+      read_v<D>(v, ring + SLOT * 2 * TILE + TILE);
       __builtin_amdgcn_sched_barrier(0);
       if (more) scores();
       add_pv(st, v, p);
+    };
+    static_assert(kRing == 4, "four steps a turn");
+    for (int j = 0; j < n; j += kRing) {
+      step(j, std::integral_constant<int, 0>{});
+      if (j + 1 < n) step(j + 1, std::integral_constant<int, 1>{});
+      if (j + 2 < n) step(j + 2, std::integral_constant<int, 2>{});
+      if (j + 3 < n) step(j + 3, std::integral_constant<int, 3>{});
     }
     st.l = row_sum(st.l);
     __syncthreads();
