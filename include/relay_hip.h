@@ -547,6 +547,10 @@ int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, const void* 
 size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_members, int max_shared, int max_own, int heads,
                                   int kv_heads, int head_dim);
 
+/* 1 where sharing is measured to be faster than rh_paged_decode_attention on the same dec_meta (whose
+ * fourth values that ignores) and tables, if every token's own table holds its whole context. */
+int rh_shared_prefix_pays(int n_dec, int max_shared, int max_own, int heads, int kv_heads, int head_dim);
+
 /* Host-side: which tokens of a step share a prefix. tokens [n_dec][4] are rh_paged_decode_attention's
  * descriptors (row, context, table offset, unused) and tables their block tables, both in host
  * memory. Writes the descriptors in the order of their groups, with their shared keys, to dec_meta

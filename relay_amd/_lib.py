@@ -116,6 +116,7 @@ SIGNATURES = {
     "rh_qk_norm_to_cache": (I, [P, I, P, I, P, P, P, F, P, P, P, P, P, P, F, I, I, I, I, P]),
     "rh_shared_prefix_attention": (I, [P, I64, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, P, SZ, P, I64, P]),
     "rh_shared_prefix_workspace": (SZ, [I, I, I, I, I, I, I, I]),
+    "rh_shared_prefix_pays": (I, [I, I, I, I, I, I]),
     "rh_shared_prefix_groups": (I, [P, P, I, I, I, P, P, P]),
     "rh_process_logits": (I, [P, I64, I, I, P, I64, P, P, P, P, P, P, P, I64, P, P, I64, P, P, I64, P, P, SZ, P]),
     "rh_process_logits_workspace": (SZ, [I, I]),

@@ -356,6 +356,12 @@ struct KvStep {
   half8 k[2][D / 32], v[kStep * (D / 8) / kWave];
 };
 
+// Two floats, coherent across the device's XCDs (as coherent_load).
+__device__ __forceinline__ float2 coherent_load2(const float* p) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return __builtin_bit_cast(float2, v);
+}
+
 // Swizzle of a key's 16-byte chunks in the staging rows.
 template <int D>
 __device__ __forceinline__ int vswz(int key) {
@@ -370,6 +376,7 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
   const scalar_ints entries = (scalar_ints)(sh.table);
   half_t* const sv = reinterpret_cast<half_t*>(smem) + w * kStep * D;
   float* const s_ml = reinterpret_cast<float*>(smem + kWaves * kFew * D * 4);  // [wave][16 rows][max, sum]
+  __shared__ int s_last[kFew], s_row[kFew];
 
   // A tile has the heads of whole tokens, or up to 16 of one token's.
   const int each = max(1, kFew / G), pieces = (G + kFew - 1) / kFew;
@@ -435,6 +442,14 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
     lookup(k0);
     if (k0 < end) issue(ahead[0], k0);
     const int4 m = a.meta[token];
+    // For the join, a thread for each token of the tile: how many slices it has, and its row.
+    int slices = 0;
+    if (JOIN && static_cast<int>(threadIdx.x) < here) {
+      const int4 mt = a.meta[token0 + threadIdx.x];
+      s_row[threadIdx.x] = mt.x;
+      if (mt.y > 0)
+        slices = parts_of(mt.w, a.shared_slice, a.shared_parts) + parts_of(mt.y - max(mt.w, 0), a.own_slice, a.own_parts);
+    }
     const int lim = on ? min(m.y, end) : end;
     half8 qb[KH];
 #pragma unroll
@@ -544,54 +559,56 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
     if constexpr (JOIN) {
       // The last workgroup of a token's slices to come joins them. Its own stores are done before the
       // barrier, so before it counts itself; the values travel by coherent stores and loads.
-      int* const s_last = reinterpret_cast<int*>(s_ml);
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
       if (static_cast<int>(threadIdx.x) < here) {
-        const int t = token0 + threadIdx.x;
-        const int4 mt = a.meta[t];
         int last = 0;
-        if (mt.y > 0) {
-          const int of = pieces * (parts_of(mt.w, a.shared_slice, a.shared_parts) + parts_of(mt.y - max(mt.w, 0), a.own_slice, a.own_parts));
-          int* const count = a.counters + (static_cast<int64_t>(t) * a.kv_heads + sh.kvh) * a.counter_step;
-          last = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of - 1 ? of / pieces : 0;
-          if (last) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (slices) {
+          int* const count = a.counters + (static_cast<int64_t>(token0 + threadIdx.x) * a.kv_heads + sh.kvh) * a.counter_step;
+          if (__hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == pieces * slices - 1) {
+            last = slices;
+            __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
         }
         s_last[threadIdx.x] = last;
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < here * G * DR; i += kThreads) {
-        const int t = token0 + i / (G * DR), d = i % DR, hd = sh.kvh * G + i / DR % G;
-        const int parts = s_last[t - token0];
+      // Two values a thread, slices' loads kMerge at a time.
+      for (int i = threadIdx.x; i < here * G * (DR / 2); i += kThreads) {
+        const int t = i / (G * (DR / 2)), d = 2 * (i % (DR / 2)), hd = sh.kvh * G + i / (DR / 2) % G;
+        const int parts = s_last[t];
         if (!parts) continue;
-        const int64_t at = (static_cast<int64_t>(t) * a.heads + hd) * most;
-        float M = -INFINITY, L = 0.0f, O = 0.0f;
+        const int64_t at = (static_cast<int64_t>(token0 + t) * a.heads + hd) * most;
+        float M = -INFINITY, L = 0.0f, O0 = 0.0f, O1 = 0.0f;
         for (int p0 = 0; p0 < parts; p0 += kMerge) {
-          float mv[kMerge], lv[kMerge], ov[kMerge], top = M;
+          float2 ml[kMerge], ov[kMerge];
+          float top = M;
 #pragma unroll
           for (int j = 0; j < kMerge; ++j) {
             if (p0 + j < parts) {
-              mv[j] = coherent_load(a.part_ml + 2 * (at + p0 + j));
-              lv[j] = coherent_load(a.part_ml + 2 * (at + p0 + j) + 1);
-              ov[j] = coherent_load(a.part_o + (at + p0 + j) * DR + d);
+              ml[j] = coherent_load2(a.part_ml + 2 * (at + p0 + j));
+              ov[j] = coherent_load2(a.part_o + (at + p0 + j) * DR + d);
             }
           }
 #pragma unroll
           for (int j = 0; j < kMerge; ++j)
-            if (p0 + j < parts) top = fmaxf(top, mv[j]);
+            if (p0 + j < parts) top = fmaxf(top, ml[j].x);
           const float base = top == -INFINITY ? 0.0f : top, keep = fast_exp2(M - base);
-          L *= keep, O *= keep;
+          L *= keep, O0 *= keep, O1 *= keep;
 #pragma unroll
           for (int j = 0; j < kMerge; ++j) {
             if (p0 + j < parts) {
-              const float f = fast_exp2(mv[j] - base);
-              L += f * lv[j];
-              O += f * ov[j];
+              const float f = fast_exp2(ml[j].x - base);
+              L += f * ml[j].y;
+              O0 += f * ov[j].x;
+              O1 += f * ov[j].y;
             }
           }
           M = top;
         }
-        a.out[a.meta[t].x * a.out_stride + static_cast<int64_t>(hd) * DR + d] = static_cast<half_t>(O / L);
+        half_t* const out = a.out + s_row[t] * a.out_stride + static_cast<int64_t>(hd) * DR + d;
+        out[0] = static_cast<half_t>(O0 / L);
+        out[1] = static_cast<half_t>(O1 / L);
       }
     }
     __syncthreads();
@@ -772,6 +789,18 @@ Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_o
 }  // namespace relay_hip
 
 using namespace relay_hip;
+
+extern "C" int rh_shared_prefix_pays(int n_dec, int max_shared, int max_own, int heads, int kv_heads, int head_dim) {
+  if (n_dec <= 0 || max_shared <= 0 || max_own < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
+  // What each token reads by itself, of which all but one reading of a prefix come from the caches: up to 100
+  // MB the decode kernel's one launch and smaller steps win. Measured (us, decode / shared; members x shared +
+  // own): 32/8 heads of 128, 4 x 4096 + 300 (70 MB) 15.1 / 18.6, 16 x 1024 + 200 (76) 14.3 / 16.2, 32 x 1024 + 300
+  // (160) 28 / 22, 32 x 4096 + 300 (562) 58 / 26; 32/4 of 64, 32 x 1024 + 300 (40) 10.3 / 13.6, 32 x 4096 + 300 (141)
+  // 18.4 / 18.2, 64 x 2048 + 500 (156) 21 / 18; 9/3 of 64, 64 x 512 + 100 (28) 11.7 / 11.8, 32 x 4096 + 300 (106) 21 / 16.
+  // 16 query heads of 128 a kv head merge slowly there: 16/1, 2 x 4096 + 100 23 / 16, 64 x 512 + 100 13.5 / 15.5.
+  const double alone = static_cast<double>(n_dec) * kv_heads * head_dim * 4 * (max_shared + 0.65 * max_own);
+  return alone > 100e6 || static_cast<int64_t>(heads / kv_heads) * head_dim > 1024;
+}
 
 extern "C" int rh_shared_prefix_groups(const int* tokens, const int* tables, int n_dec, int block_size, int min_shared,
                                        int* dec_meta, int* groups, int* limits) {

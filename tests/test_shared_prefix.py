@@ -197,9 +197,10 @@ def test_row_strides(torch_mod, dev):
 
 
 @gpu
-def test_unwritten_slots_are_not_read(torch_mod, dev):
-    """NaN and infinities in the slots behind every context."""
-    case = Case([(3, 50)], [21, 2], 8, 2, 64, seed=8)
+@pytest.mark.parametrize("members,shared,D", [(3, 50, 64), (9, 50, 64), (9, 50, 128), (3, 1100, 32), (40, 333, 64)])
+def test_unwritten_slots_are_not_read(torch_mod, dev, members, shared, D):
+    """NaN and infinities in the slots behind every context and every prefix."""
+    case = Case([(members, shared)], [21, 2], 8, 2, D, seed=8)
     used = {w for rows in case.keys for w in rows}
     for b in range(case.k.shape[0]):
         for s in range(case.bs):
@@ -207,6 +208,26 @@ def test_unwritten_slots_are_not_read(torch_mod, dev):
                 case.k[b, :, s] = 0x7E00  # NaN
                 case.v[b, :, s] = 0x7C00 if s % 2 else 0x7E00
     check(torch_mod, dev, case)
+
+
+@gpu
+@pytest.mark.parametrize("groups", [[(3, 80), (1, 0)], [(12, 300)]])
+def test_cache_past_four_giga_values(torch_mod, dev, groups):
+    """Blocks behind 2^32 values of K and of V: offsets need 64 bits."""
+    torch = torch_mod
+    case = Case(groups, [40, 5], 16, 8, 128, seed=14)
+    call = Call(torch, dev, case)
+    far, per = 262144 + 3, 8 * 16 * 128
+    pools = [torch.empty((far + case.k.shape[0]) * per, dtype=torch.int16, device=dev) for _ in range(2)]
+    for pool, small in zip(pools, (call.k, call.v)):
+        pool[far * per:] = small.reshape(-1)
+    args = list(call.args)
+    args[2], args[3] = pools[0].data_ptr(), pools[1].data_ptr()
+    call.tables += far
+    _lib.check(call.lib.rh_shared_prefix_attention(*args, None))
+    torch.cuda.synchronize()
+    want, tol = case.oracle()
+    assert (np.abs(call.out.double().cpu().numpy() - want) <= tol).all()
 
 
 @gpu
@@ -368,6 +389,13 @@ def test_refusals(change, message):
     lib = _lib.lib()
     assert lib.rh_shared_prefix_attention(*{**GOOD, **change}.values()) != 0
     assert message in _lib.last_error()
+
+
+@pytest.mark.parametrize("n,shared,own,heads,kv_heads,D,pays", [
+    (4, 4096, 300, 32, 8, 128, 0), (32, 1024, 300, 32, 8, 128, 1), (64, 16384, 1000, 32, 8, 128, 1), (32, 2048, 300, 32, 4, 64, 0), (64, 2048, 500, 32, 4, 64, 1),
+    (2, 512, 40, 9, 3, 64, 0), (2, 4096, 100, 16, 1, 128, 1), (64, 0, 9000, 32, 8, 128, 0), (0, 512, 40, 9, 3, 64, 0), (4, 512, 40, 9, 2, 64, 0)])
+def test_sharing_pays_where_it_is_measured_faster(n, shared, own, heads, kv_heads, D, pays):
+    assert _lib.lib().rh_shared_prefix_pays(n, shared, own, heads, kv_heads, D) == pays
 
 
 def test_nothing_to_do_is_not_an_error():

@@ -267,6 +267,25 @@ def test_qk_norm_far_positions_and_extremes(torch_mod, dev):
 
 
 @gpu
+def test_qk_norm_into_a_cache_past_four_giga_values(torch_mod, dev):
+    """A slot behind 2^32 values of each pool."""
+    torch = torch_mod
+    case = QkCase(3, 9, 8, 128, seed=7)
+    far = 262144 + 5
+    pools = [torch.empty(far + case.nb, 8, 16, 128, dtype=torch.float16, device=dev) for _ in range(2)]
+    for pool, small in zip(pools, case.pool):
+        pool[far:] = dev_of(torch, dev, small)
+    d = lambda a: dev_of(torch, dev, a)  # noqa: E731
+    t = [d(case.qkv), d(case.wq), d(case.wk), d(case.inv_freq), dev_of(torch, dev, case.pos, np.int32), dev_of(torch, dev, case.slot + far * 16, np.int32), d(case.q0)]
+    _lib.check(_lib.lib().rh_qk_norm_to_cache(ptr(t[0]), 1, None, 3, None, ptr(t[1]), ptr(t[2]), case.eps, ptr(t[3]), ptr(t[4]), ptr(t[5]), ptr(pools[0]),
+                                              ptr(pools[1]), ptr(t[6]), case.q_scale, 9, 8, 128, 16, None))
+    torch.cuda.synchronize()
+    for name, pool in zip("kv", pools):
+        want, tol = case.oracle()[name]
+        assert (np.abs(pool[far:].cpu().numpy().astype(np.float64) - want) <= tol).all()
+
+
+@gpu
 def test_qk_norm_many_rows(torch_mod, dev):
     check_qk(torch_mod, dev, QkCase(1501, 8, 2, 64, seed=5, idle=(3, 1500)))
     check_qk(torch_mod, dev, QkCase(700, 32, 8, 128, seed=6, planes=2))
