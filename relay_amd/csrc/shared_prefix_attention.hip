@@ -40,6 +40,18 @@ constexpr int kFew = 16;   // query rows of a workgroup whose waves take keys of
 constexpr int kMerge = 8;  // slices whose values are loaded at once (attend_few)
 constexpr int kRing = 4;    // 32-key tiles of K and V in LDS, where strips share them
 
+// n / d for 0 <= n < limit by one multiplication (m = ceil(2^32 / d) is exact while n * d < 2^32; else m is 0
+// and the division is made): an integer division is some 40 instructions, and a workgroup's place takes six.
+struct Div {
+  unsigned d, m;
+  __device__ __forceinline__ int operator()(int n) const {
+    return d == 1 ? n : m ? static_cast<int>(__umulhi(static_cast<unsigned>(n), m)) : static_cast<int>(static_cast<unsigned>(n) / d);
+  }
+};
+Div div_by(int d, int64_t limit) {
+  return {static_cast<unsigned>(d), d > 1 && limit * d < (int64_t{1} << 32) ? static_cast<unsigned>(((int64_t{1} << 32) + d - 1) / d) : 0u};
+}
+
 struct SharedArgs {
   const half_t* q;
   int64_t q_stride;
@@ -50,6 +62,8 @@ struct SharedArgs {
   int n_dec, n_groups, heads, kv_heads, group, block, bs_shift;
   int shared_slice, shared_parts, own_slice, own_parts, tiles, own_tiles;  // tiles: row tiles of a group, of a token
   int shared_units, shared_wgs, own_units;  // workgroups on prefixes come first
+  int each, pieces;  // attend_few: tokens of a row tile, row tiles of a token (one of the two is 1)
+  Div by_tiles, by_own_tiles, by_shared_parts, by_own_parts, by_kv_heads, by_group;  // (by_group: rows of attend_few)
   float scale_log2;
   int* counters;  // per token and kv head, counter_step apart: slices that have come (zero between calls)
   int counter_step;
@@ -61,11 +75,6 @@ struct SharedArgs {
 // Slices of `keys` keys where the launch has room for `most`; the last takes what is left.
 __device__ __forceinline__ int parts_of(int keys, int slice, int most) {
   return keys <= 0 ? 0 : min(most, (keys + slice - 1) / slice);
-}
-
-// Row tiles of kFew of some tokens (attend_few).
-__device__ __host__ __forceinline__ int64_t tiles_few(int64_t members, int group) {
-  return group <= kFew ? (members + kFew / group - 1) / (kFew / group) : members * ((group + kFew - 1) / kFew);
 }
 
 __device__ __forceinline__ float row_max(float x) {
@@ -379,16 +388,17 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
   __shared__ int s_last[kFew], s_row[kFew];
 
   // A tile has the heads of whole tokens, or up to 16 of one token's.
-  const int each = max(1, kFew / G), pieces = (G + kFew - 1) / kFew;
-  for (; sh.tile < tiles_few(sh.members, G); sh.tile += sh.step) {
+  const int each = a.each, pieces = a.pieces;
+  for (; pieces == 1 ? sh.tile * each < sh.members : sh.tile < sh.members * pieces; sh.tile += sh.step) {
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
     const int c = lane & 15, g = lane >> 4;
-    const int token0 = sh.first + sh.tile / pieces * each, head0 = sh.tile % pieces * kFew;
+    const int whole = pieces == 1 ? sh.tile : sh.tile / pieces;
+    const int token0 = sh.first + whole * each, head0 = (sh.tile - whole * pieces) * kFew;
     const int here = min(each, sh.first + sh.members - token0);  // tokens of the tile
     const int rows = here * min(G - head0, kFew);
-    const auto token_of = [&](int row) { return token0 + (pieces == 1 ? row / G : 0); };
-    const auto head_of = [&](int row) { return sh.kvh * G + (pieces == 1 ? row % G : head0 + row); };
+    const auto token_of = [&](int row) { return token0 + (pieces == 1 ? a.by_group(row) : 0); };
+    const auto head_of = [&](int row) { return sh.kvh * G + (pieces == 1 ? row - a.by_group(row) * G : head0 + row); };
     const auto row_any = [&](int j) -> unsigned {
       j = min(j, end - 1);
       return (static_cast<unsigned>(sh.table[bshift >= 0 ? j >> bshift : j / bs]) * a.kv_heads + sh.kvh) * bs +
@@ -575,7 +585,7 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
       __syncthreads();
       // Two values a thread, slices' loads kMerge at a time.
       for (int i = threadIdx.x; i < here * G * (DR / 2); i += kThreads) {
-        const int t = i / (G * (DR / 2)), d = 2 * (i % (DR / 2)), hd = sh.kvh * G + i / (DR / 2) % G;
+        const int row = i / (DR / 2), t = pieces == 1 ? a.by_group(row) : 0, d = 2 * (i % (DR / 2)), hd = sh.kvh * G + row - t * G;
         const int parts = s_last[t];
         if (!parts) continue;
         const int64_t at = (static_cast<int64_t>(token0 + t) * a.heads + hd) * most;
@@ -630,13 +640,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D > 64
   int b = shared ? blockIdx.x : blockIdx.x - a.shared_wgs;
   Share g;
   g.step = shared ? a.tiles : a.own_tiles;
-  g.tile = (b >> 3) % g.step;
-  b = (b >> 3) / g.step * 8 + (b & 7);
+  const int over = shared ? a.by_tiles(b >> 3) : a.by_own_tiles(b >> 3);
+  g.tile = (b >> 3) - over * g.step;
+  b = over * 8 + (b & 7);
   if (b >= (shared ? a.shared_units : a.own_units)) return;
   if (shared) {
-    g.part = b % a.shared_parts, b /= a.shared_parts;
-    g.kvh = b % a.kv_heads;
-    const int4 rec = a.groups[b / a.kv_heads];
+    const int head = a.by_shared_parts(b), group = a.by_kv_heads(head);
+    g.part = b - head * a.shared_parts;
+    g.kvh = head - group * a.kv_heads;
+    const int4 rec = a.groups[group];
     const int parts = parts_of(rec.z, a.shared_slice, a.shared_parts);
     if (g.part >= parts) return;
     g.first = rec.x, g.members = rec.y, g.table = a.tables + rec.w;
@@ -647,9 +659,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D > 64
       return;
     }
   } else {
-    g.part = b % a.own_parts, b /= a.own_parts;
-    g.kvh = b % a.kv_heads;
-    g.first = b / a.kv_heads, g.members = 1;
+    const int head = a.by_own_parts(b);
+    g.part = b - head * a.own_parts;
+    g.first = a.by_kv_heads(head), g.members = 1;
+    g.kvh = head - g.first * a.kv_heads;
     const int4 m = a.meta[g.first];
     const int from = max(m.w, 0), parts = parts_of(m.y - from, a.own_slice, a.own_parts);
     if (g.part >= parts) return;
@@ -746,9 +759,10 @@ Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_o
   // one has more slices than one workgroup joins well. Measured (us, so / as many rows): 6 rows on 512
   // keys 9.0 / 10.8, 8 on 4096 at head size 128 21 / 18, 16 on 16,384 48 / 31; 24 on 1024 13.6 / 11.3.
   p.rows = pieces && (rows > kFew || max_shared > 1024);
-  const int64_t tiles = p.rows ? (rows + kWaves * kStrip - 1) / (kWaves * kStrip) : tiles_few(max_members, group);
+  const int each = std::max(1, kFew / group), pieces_of = (group + kFew - 1) / kFew;
+  const int64_t tiles = p.rows ? (rows + kWaves * kStrip - 1) / (kWaves * kStrip) : (static_cast<int64_t>(max_members) + each - 1) / each * pieces_of;
   p.tiles = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), 1 << 20));
-  p.own_tiles = static_cast<int>(tiles_few(1, group));
+  p.own_tiles = pieces_of;
   // Slices of multiples of 128 keys, by what a launch of them takes (us, measured on MI355X): a start of
   // 5, a step of 32 keys of 128 rows 1.05 at head size 128 and 0.5 below, of 128 own keys 1.5 and 0.8,
   // in rounds of the workgroups that the card holds, and each slice's way through memory to its
@@ -939,6 +953,14 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   a.shared_units = static_cast<int>(shared_units);
   a.own_units = static_cast<int>(own_units);
   a.shared_wgs = static_cast<int>(shared_wgs);
+  a.each = std::max(1, kFew / a.group);
+  a.pieces = (a.group + kFew - 1) / kFew;
+  a.by_tiles = div_by(p.tiles, wgs);
+  a.by_own_tiles = div_by(p.own_tiles, wgs);
+  a.by_shared_parts = div_by(p.shared_parts, wgs);
+  a.by_own_parts = div_by(p.own_parts, wgs);
+  a.by_kv_heads = div_by(kv_heads, wgs);
+  a.by_group = div_by(a.group, std::max(kFew, a.each * a.group) + 1);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (head_dim) {
     case 16: if (int rc = launch<32, 16>(a, p.rows, wgs, s)) return rc; break;
