@@ -756,9 +756,10 @@ Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_o
   // Shared tiles come in pieces of up to 16 keys of one block, straight to LDS.
   const bool pieces = head_dim > 16 && block >= 16 && (block & (block - 1)) == 0;
   // Few rows on a short prefix are joined by the last workgroup that comes, which saves a launch; a long
-  // one has more slices than one workgroup joins well. Measured (us, so / as many rows): 6 rows on 512
-  // keys 9.0 / 10.8, 8 on 4096 at head size 128 21 / 18, 16 on 16,384 48 / 31; 24 on 1024 13.6 / 11.3.
-  p.rows = pieces && (rows > kFew || max_shared > 1024);
+  // one has more slices than one workgroup joins well, and many values take it long. Measured (us, so / as
+  // many rows): 6 rows on 512 keys at head size 64 7.7 / 10.2, 15 there 9.4 / 10.4; 12 on 512 at head size
+  // 128 12.4 / 12.6, 16 there 13.9 / 12.8; 8 on 4096 at 128 21 / 18; 24 on 1024 at 64 13.6 / 11.3.
+  p.rows = pieces && (rows > kFew || rows * head_dim > 1536 || max_shared > 1024);
   const int each = std::max(1, kFew / group), pieces_of = (group + kFew - 1) / kFew;
   const int64_t tiles = p.rows ? (rows + kWaves * kStrip - 1) / (kWaves * kStrip) : (static_cast<int64_t>(max_members) + each - 1) / each * pieces_of;
   p.tiles = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), 1 << 20));
