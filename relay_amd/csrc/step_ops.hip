@@ -385,6 +385,7 @@ __device__ __forceinline__ unsigned long long token_key(float x, int token) {
   return static_cast<unsigned long long>(k) << 32 | (0xffffffffu - static_cast<unsigned>(token));
 }
 
+template <int THREADS>
 __device__ __forceinline__ unsigned long long block_best(unsigned long long v, unsigned long long* waves) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -395,29 +396,35 @@ __device__ __forceinline__ unsigned long long block_best(unsigned long long v, u
   __syncthreads();
   v = waves[0];
 #pragma unroll
-  for (int i = 1; i < kThreads / 64; ++i) v = waves[i] > v ? waves[i] : v;
+  for (int i = 1; i < THREADS / 64; ++i) v = waves[i] > v ? waves[i] : v;
   __syncthreads();
   return v;
 }
 
 // BIAS: there are biases. VEC: a row's logits and results lie alike to 16 bytes.
-template <bool BIAS, bool VEC, int kVec>
-__global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArgs a) {
+template <bool BIAS, bool VEC, int kVec, int THREADS>
+__global__ __launch_bounds__(THREADS) void process_logits_kernel(const LogitArgs a) {
   // A word for each logit of the slice: first what the history says, then the last bias that names it
   // (an array of its own for these would halve the workgroups that a CU holds: 64 rows of 128,257
   // 32 / 30 us).
-  constexpr int kSlice = 4 * kVec * kThreads;
+  constexpr int kSlice = 4 * kVec * THREADS;
   __shared__ __attribute__((aligned(16))) unsigned s_word[kSlice];
-  __shared__ unsigned long long s_best[kThreads / 64];
+  __shared__ unsigned long long s_best[THREADS / 64];
   __shared__ int s_last;
-  const int row = blockIdx.x / a.slices, part = blockIdx.x % a.slices;
+  // Workgroups go round the 8 XCDs; a row's go to one, whose L2 then serves its history (as many rows as come in
+  // eights; 64 rows of 32,000 with histories of 8000 15 / 13.8 us, of 128,257 with 100 level).
+  int row = blockIdx.x / a.slices, part = blockIdx.x % a.slices;
+  if (row < (a.rows & ~7)) {
+    const int over = (blockIdx.x >> 3) / a.slices;
+    row = 8 * over + (blockIdx.x & 7), part = (blockIdx.x >> 3) - over * a.slices;
+  }
   const float* in = a.in + row * a.ld;
   float* out = a.out + row * a.out_ld;
   // The slice's first logit; the first slice begins up to three before the row.
   const int v0 = part * kSlice - (VEC ? static_cast<int>(reinterpret_cast<uintptr_t>(in) / 4 % 4) : 0);
-  const auto at = [&](int i) { return VEC ? 4 * (threadIdx.x + i * kThreads) : static_cast<int>(threadIdx.x) + 4 * i * kThreads; };
-  // The first tokens of the history, kAhead pieces of four a thread (rows begin at any word), before the
-  // logits: loads return in order, and the history is worked on while the logits come.
+  const auto at = [&](int i) { return VEC ? 4 * (threadIdx.x + i * THREADS) : static_cast<int>(threadIdx.x) + 4 * i * THREADS; };
+  // The history in pieces of four tokens a thread (rows begin at any word), kAhead of them in flight and the first
+  // before the logits: loads return in order, and the history is worked on while the logits come.
   constexpr int kAhead = 4;
   struct __attribute__((packed, aligned(4))) Four {
     int token[4];
@@ -426,20 +433,18 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
   const int prompt = a.prompt_len ? a.prompt_len[row] : 0;
   const int* h = a.history + row * a.history_stride;
   Four said[kAhead];
-  const auto tokens_from = [&](int j0) {
+  const auto tokens_at = [&](int i, int j0) {  // piece i from token j0 on, the same for all threads
+    const int j = j0 + 4 * static_cast<int>(threadIdx.x);
+    if (j0 >= len) return;
+    if (j + 3 < len) {
+      said[i] = *reinterpret_cast<const Four*>(h + j);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int j = j0 + 4 * i * kThreads;
-      if (j - 4 * static_cast<int>(threadIdx.x) >= len) break;  // the same for all threads
-      if (j + 3 < len) {
-        said[i] = *reinterpret_cast<const Four*>(h + j);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) said[i].token[e] = j + e < len ? h[j + e] : -1;
-      }
+      for (int e = 0; e < 4; ++e) said[i].token[e] = j + e < len ? h[j + e] : -1;
     }
   };
-  tokens_from(4 * threadIdx.x);
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) tokens_at(i, 4 * i * THREADS);
   float x[kVec][4];
 #pragma unroll
   for (int i = 0; i < kVec; ++i) {
@@ -450,7 +455,7 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int u = v + (VEC ? e : e * kThreads);
+        const int u = v + (VEC ? e : e * THREADS);
         x[i][e] = u >= 0 && u < a.vocab ? in[u] : 0.0f;
       }
     }
@@ -472,17 +477,17 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
   }
   const auto clear = [&] {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) reinterpret_cast<uint4v*>(s_word)[threadIdx.x + i * kThreads] = uint4v{0, 0, 0, 0};
+    for (int i = 0; i < kVec; ++i) reinterpret_cast<uint4v*>(s_word)[threadIdx.x + i * THREADS] = uint4v{0, 0, 0, 0};
     __syncthreads();
   };
   // A thread's words, laid out as its logits are.
   const auto words_of = [&](int i, unsigned (&w)[4]) {
     if (VEC) {
-      const uint4v s = reinterpret_cast<const uint4v*>(s_word)[threadIdx.x + i * kThreads];
+      const uint4v s = reinterpret_cast<const uint4v*>(s_word)[threadIdx.x + i * THREADS];
       w[0] = s[0], w[1] = s[1], w[2] = s[2], w[3] = s[3];
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = s_word[at(i) + e * kThreads];
+      for (int e = 0; e < 4; ++e) w[e] = s_word[at(i) + e * THREADS];
     }
   };
   // A token's place among the slice's from its first in the vocabulary on: n and more for any other token, one
@@ -494,22 +499,23 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
     const float rep = a.repetition ? a.repetition[row] : 1.0f;
     const float freq = a.frequency ? a.frequency[row] : 0.0f, pres = a.presence ? a.presence[row] : 0.0f;
     clear();
-    for (int j0 = 4 * threadIdx.x; j0 - 4 * static_cast<int>(threadIdx.x) < len; j0 += 4 * kAhead * kThreads) {
+    for (int j0 = 0; j0 < len; j0 += 4 * kAhead * THREADS) {
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        if (j0 - 4 * static_cast<int>(threadIdx.x) + 4 * i * kThreads >= len) break;
+        const int j = j0 + 4 * i * THREADS;
+        if (j >= len) break;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const unsigned p = place(said[i].token[e]);
           if (p < n) {
-            if (j0 + 4 * i * kThreads + e < prompt)
+            if (j + 4 * static_cast<int>(threadIdx.x) + e < prompt)
               atomicOr(&words[p], 0x80000000u);
             else
               atomicAdd(&words[p], 1u);
           }
         }
+        tokens_at(i, j + 4 * kAhead * THREADS);
       }
-      tokens_from(j0 + 4 * kAhead * kThreads);
     }
     __syncthreads();
 #pragma unroll
@@ -531,10 +537,10 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
   if (BIAS && biases > 0) {
     __syncthreads();  // the history's words have been read
     clear();
-    for (int j = threadIdx.x; j < biases; j += kThreads) {
+    for (int j = threadIdx.x; j < biases; j += THREADS) {
       const unsigned p = place(named);
       if (p < n) atomicMax(&words[p], static_cast<unsigned>(j + 1));
-      named = j + kThreads < biases ? a.bias_tokens[bias_at + j + kThreads] : -1;
+      named = j + THREADS < biases ? a.bias_tokens[bias_at + j + THREADS] : -1;
     }
     __syncthreads();
 #pragma unroll
@@ -552,7 +558,7 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
     const int v = v0 + at(i);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int u = v + (VEC ? e : e * kThreads);
+      const int u = v + (VEC ? e : e * THREADS);
       if (u >= 0 && u < a.vocab) {
         const unsigned word = !VEC ? (mask_row >= 0 ? mask[u >> 5] : ~0u) : u >> 5 == max(v, 0) >> 5 ? lo[i] : hi[i];
         if (!((word >> (u & 31)) & 1u)) x[i][e] = -INFINITY;
@@ -563,7 +569,7 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
   }
   unsigned long long* const record = a.records + row * a.record;
   if (a.next) {
-    best = block_best(best, s_best);
+    best = block_best<THREADS>(best, s_best);
     if (threadIdx.x == 0) {
       __hip_atomic_store(&record[1 + part], best, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __builtin_amdgcn_s_waitcnt(0);
@@ -578,7 +584,7 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int u = v + (VEC ? e : e * kThreads);
+        const int u = v + (VEC ? e : e * THREADS);
         if (u >= 0 && u < a.vocab) out[u] = x[i][e];
       }
     }
@@ -588,21 +594,25 @@ __global__ __launch_bounds__(kThreads) void process_logits_kernel(const LogitArg
   if (!s_last) return;
   // The row's last workgroup takes the best of all slices and leaves the record zero again, for calls of any shape.
   best = 0;
-  for (int p = threadIdx.x; p <= a.slices; p += kThreads) {
+  for (int p = threadIdx.x; p <= a.slices; p += THREADS) {
     const unsigned long long k = __hip_atomic_load(&record[p], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __hip_atomic_store(&record[p], 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (p) best = k > best ? k : best;
   }
-  best = block_best(best, s_best);
+  best = block_best<THREADS>(best, s_best);
   if (threadIdx.x == 0) a.next[row] = best ? static_cast<int>(0xffffffffu - static_cast<unsigned>(best)) : -1;
 }
 
-// Logits of a workgroup: one 16-byte load a thread while that makes few workgroups, else two (each workgroup
-// reads its row's whole history). Measured (us, histories of 2000, one / two / four loads): 1 x 32,000
-// 7.2 / 8.0 / 10.0, 8 x 128,256 9.6 / 9.0 / 10.7, 48 x 32,000 10.5 / 9.9 / 12.3, 32 x 128,256 18.6 / 14.9 / 14.7,
-// 64 x 128,257 with 8000 41 / 27.6 / 28.6, of which reading and writing the logits take 15, the token
-// 2, the biases 3 and the history 8.
-int slice_of(int rows, int vocab) { return static_cast<int64_t>(rows) * ((vocab + 1023) / 1024) <= 512 ? 1024 : 2048; }
+// Logits of a workgroup: one 16-byte load a thread while that makes few workgroups, else two. Each workgroup reads
+// its row's whole history, so where that may be long it has twice the threads. Measured (us; histories of 2000, one / two /
+// four loads of 256 threads): 1 x 32,000 7.2 / 8.0 / 10.0, 8 x 128,256 9.6 / 9.0 / 10.7, 48 x 32,000 10.5 / 9.9 / 12.3, 32 x
+// 128,256 18.6 / 14.9 / 14.7. 256 / 512 threads: 64 x 128,257 with 100 18.9 / 19.8, with 4000 23.0 / 23.4, with 8000 and 300
+// biases 27.6 / 26.2, with 16,000 31.3 / 28.1, 1 x 128,256 with 120,000 32 / 21; 1024 threads are slower by 1-15%.
+int threads_of(int64_t history_stride) { return history_stride > 4096 ? 512 : 256; }
+int slice_of(int rows, int vocab, int threads) {
+  const int one = 4 * threads;
+  return static_cast<int64_t>(rows) * ((vocab + one - 1) / one) <= 512 ? one : 2 * one;
+}
 // Slices of a row, which may begin up to three logits into its first one.
 int slices_of(int vocab, int slice) { return static_cast<int>((static_cast<int64_t>(vocab) + 3 + slice - 1) / slice); }
 
@@ -687,7 +697,7 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
 
 size_t rh_process_logits_workspace(int rows, int vocab) {
   if (rows <= 0 || vocab <= 0) return 0;
-  return static_cast<size_t>(rows) * record_words(vocab, slice_of(rows, vocab)) * 8;
+  return static_cast<size_t>(rows) * record_words(vocab, slice_of(rows, vocab, 256)) * 8;  // 512 threads have fewer slices
 }
 
 int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, const int* history, int64_t history_stride,
@@ -705,7 +715,7 @@ int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, cons
   RH_REQUIRE(!bias_tokens || (bias_values && bias_len && bias_stride >= 0 && bias_stride < kSumCap),
              "process_logits: biases need values, lengths and a stride below 2^30");
   RH_REQUIRE(!masks || mask_stride >= (static_cast<int64_t>(vocab) + 31) / 32, "process_logits: a mask row holds a bit for each token");
-  const int slice = slice_of(rows, vocab), slices = slices_of(vocab, slice);
+  const int threads = threads_of(history ? history_stride : 0), slice = slice_of(rows, vocab, threads), slices = slices_of(vocab, slice);
   RH_REQUIRE(static_cast<int64_t>(rows) * slices < (int64_t{1} << 31), "process_logits: too many rows");
   RH_REQUIRE(!next || (workspace && workspace_bytes >= rh_process_logits_workspace(rows, vocab) &&
                        reinterpret_cast<uintptr_t>(workspace) % 8 == 0),
@@ -717,11 +727,15 @@ int rh_process_logits(const float* logits, int64_t ld, int rows, int vocab, cons
   const bool vec = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(out)) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(logits) % 4 == 0 && (ld - out_ld) % 4 == 0;
   const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3(rows * slices), dim3(kThreads), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(kernel, dim3(rows * slices), dim3(threads), 0, static_cast<hipStream_t>(stream), a);
   };
   const auto of_loads = [&](auto bias, auto aligned) {
     constexpr bool B = decltype(bias)::value, V = decltype(aligned)::value;
-slice == 1024 ? go(process_logits_kernel<B, V, 1>) : go(process_logits_kernel<B, V, 2>);
+    const bool one = slice == 4 * threads;
+    if (threads == 512)
+      one ? go(process_logits_kernel<B, V, 1, 512>) : go(process_logits_kernel<B, V, 2, 512>);
+    else
+      one ? go(process_logits_kernel<B, V, 1, 256>) : go(process_logits_kernel<B, V, 2, 256>);
   };
   if (bias_tokens) {
     RH_TRY_LAUNCH(vec ? of_loads(std::true_type{}, std::true_type{}) : of_loads(std::true_type{}, std::false_type{}));

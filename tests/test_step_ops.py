@@ -419,6 +419,13 @@ def test_logits_rows(torch_mod, dev, rows):
 
 
 @gpu
+@pytest.mark.parametrize("rows,vocab,history", [(1, 1, 4097), (2, 40001, 4096), (2, 40001, 4097), (7, 5003, 9000), (8, 9001, 6001), (17, 65001, 4100),
+                                                (25, 50257, 5000)])
+def test_logits_long_histories(torch_mod, dev, rows, vocab, history):
+    check_logits(torch_mod, dev, LogitCase(rows, vocab, history, biases=600, masks=3, seed=rows + history))
+
+
+@gpu
 @pytest.mark.parametrize("shift", [0, 1, 2, 3])
 @pytest.mark.parametrize("ld,out_ld", [(4100, 4100), (4101, 4101), (4099, 4100), (4100, 5003)])
 def test_logits_strides_and_alignment(torch_mod, dev, shift, ld, out_ld):
@@ -484,6 +491,7 @@ def test_logits_calls_of_other_sizes_share_a_workspace(torch_mod, dev):
     ws = torch_mod.zeros(1 << 20, dtype=torch_mod.uint8, device=dev)
     for rows, vocab in ((3, 50000), (64, 4097), (1, 100), (33, 20000), (3, 50000)):
         check_logits(torch_mod, dev, LogitCase(rows, vocab, 20, 2, 1, seed=rows), workspace=ws)
+        check_logits(torch_mod, dev, LogitCase(rows, vocab, 4500, 2, 1, seed=rows), workspace=ws)
 
 
 @gpu
