@@ -475,7 +475,7 @@ int rh_kv_scatter_from_host(void* kpool, void* vpool, const int* blocks, int n, 
 /* Block tables and slot maps of a step, from the lengths of its sequences.
  *  cached [n_seqs]      tokens of each sequence that the cache holds
  *  fresh  [n_seqs]      tokens that this step adds (0: the sequence waits)
- *  shared [n_seqs]      leading keys that its group shares (NULL: none)
+ *  shared [n_seqs]      leading keys that its group shares, which are in the cache (NULL: none)
  *  group_seqs [n_groups][2]  first sequence and number of sequences of each group
  *  tables [n_seqs][table_stride]  block ids; sequence s holds ceil(cached[s] / block_size) on
  *                       entry and ceil((cached[s] + fresh[s]) / block_size) afterwards
@@ -530,8 +530,9 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
  *                        of the table that the shared keys are read through
  * A token attends to keys 0 .. context - 1: those below its shared keys through its group's table,
  * the others through its own. It belongs to exactly one group if its shared keys are positive, and
- * they are the group's; its context may end before them. A token of context 0 is idle, its row
- * left as it was. Several tokens of one sequence are several entries.
+ * they are the group's. A group's table holds all its shared keys, written and finite; a member's
+ * context may end before them. A token of context 0 is idle, its row left as it was. Several
+ * tokens of one sequence are several entries, each with a row of its own.
  *  max_members, max_shared, max_own  the largest group, the most shared keys and the most keys
  *                        behind them: they choose how the work is cut. Beyond them results stay
  *                        right and the call gets slower

@@ -9,16 +9,17 @@
 // for the product with V, as in the other attention kernels: an MFMA operand of twice the width
 // would double that product. Two ways through a slice:
 //
-//  - many rows (prefixes of more than 16 rows or 1024 keys): 128 rows, 32 a wave, on tiles of K and V that
-//    the waves share in LDS (attend_rows). Bound by the chain of a step (LDS reads, products, weights:
-//    no one of them taken out made it faster by over a tenth) and by K and V from memory.
+//  - many rows (prefixes of more than 16 rows or 1024 keys, or of more than 12 rows of 128): 128 rows, 32 a
+//    wave, on tiles of K and V that the waves share in LDS (attend_rows). 64 x 4 rows on 16,384 keys of
+//    8 heads of 128 take 35.5 us (17 GFLOP, 67 MB). Bound by the chain of a step (LDS reads, products,
+//    weights: no one of them taken out made it faster by over a tenth) and by K and V from memory.
 //  - few rows (own keys, short prefixes): 16 rows, the waves on keys of their own, K straight into MFMA
-//    operands (attend_few). Bound by memory: 64 x 1000 own keys, 8 kv heads of 128 (ragged, 164 MB) 40 us.
+//    operands (attend_few). Bound by memory: 64 x 1000 own keys, 8 kv heads of 128 (ragged, 164 MB) 39 us.
 //
 // One launch does both, prefixes first: the prefix's products run beside the own keys' loads. 64 members on
-// 16,384 keys with up to 1000 of their own (231 MB, 18 GFLOP) take 61 us, the join 7. Prefix and own keys in
-// workgroups of eight waves, one a CU, or staged through registers, whose reloads from scratch waited
-// for every load in flight, took 107.
+// 16,384 keys with up to 1000 of their own (231 MB, 18 GFLOP) take 57 us, the join 6. Prefix tiles staged
+// through registers, whose reloads from scratch waited for every load in flight, took 107 in all, and
+// workgroups of eight waves that do not share their tiles 244.
 #include <algorithm>
 #include <exception>
 #include <string>
@@ -36,8 +37,8 @@ constexpr int kStrip = 32;  // query rows of a wave: a strip
 constexpr int kStep = 32;   // keys of a wave's step
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kFew = 16;   // query rows of a workgroup whose waves take keys of their own
-constexpr int kMerge = 8;  // slices whose values are loaded at once (attend_few)
+constexpr int kFew = 16;    // query rows of a workgroup whose waves take keys of their own
+constexpr int kMerge = 8;   // slices whose values are loaded at once (attend_few)
 constexpr int kRing = 4;    // 32-key tiles of K and V in LDS, where strips share them
 
 // n / d for 0 <= n < limit by one multiplication (m = ceil(2^32 / d) is exact while n * d < 2^32; else m is 0
