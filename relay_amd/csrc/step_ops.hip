@@ -17,18 +17,20 @@ namespace {
 //
 // held = ceil(cached / B), want = ceil((cached + fresh) / B); sequence s takes want - held ids off the
 // top of the free stack, behind those of the sequences before it, and has the rows row_off[s] ..
-// row_off[s + 1] - 1: two exclusive sums over the sequences. One workgroup takes them, a sequence a
-// thread (more in several turns): they are a chain of dependent steps. Where no sequence adds more than
-// kOwnRows tokens, as in decoding, its thread writes its rows too, from what it has in registers;
-// otherwise every row finds its sequence by binary search, in a launch of its own past kOneLaunch
-// rows (48 decoding sequences 6.3 us with a search, 511 sequences of which 40 add a prompt, 26,500
-// rows, 58 us in one workgroup).
+// row_off[s + 1] - 1: two exclusive sums over the sequences, a chain of dependent steps that bounds the call.
+// Up to kWideRows rows one workgroup takes them, a sequence a thread (more in several turns); where no
+// sequence adds more than kOwnRows tokens, as in decoding, its thread writes its rows too, from what it
+// has in registers (48 decoding sequences 3.9 us, with a search for each row's sequence 6.3). Larger steps take
+// many workgroups that all make the sums (step_wide_kernel; 511 sequences of which 40 add a prompt, 26,500
+// rows, 5.5 us), unless the stack's count lies in the totals: then one workgroup makes them, with the rows in a
+// second launch past kOneLaunch of them (9.4 us; in one workgroup 58).
 
 constexpr int kSumCap = (1 << 30) - 1;  // sums stop here, past every limit that they are compared with
 constexpr int kOwnRows = 4;
+constexpr int kWideRows = 512;           // 511 decoding sequences 5.3 us in one workgroup, 5.5 in two; 48 and a prompt of 512 6.5, 4.7
 constexpr int kOneLaunch = 4096;
 constexpr int kRowThreads = 256;
-constexpr int kRowOffsets = 4096;       // row offsets that a workgroup of step_rows_kernel keeps in LDS
+constexpr int kRowOffsets = 4096;        // sequences whose first rows a workgroup keeps in LDS
 
 struct StepArgs {
   const int *cached, *fresh, *shared, *group_seqs;
@@ -72,6 +74,43 @@ __device__ Need block_scan(Need v, Need* waves, Need* total) {
   }
   *total = sum;
   return {capped_add(before.rows, v.rows), capped_add(before.blocks, v.blocks)};
+}
+
+struct Length {
+  int cached, shared, bad;
+  Need need;
+};
+
+// What sequence s adds, or why it cannot.
+__device__ __forceinline__ Length length_of(const StepArgs& a, int s) {
+  Length n{a.cached[s], a.shared ? a.shared[s] : 0, 0, {0, 0}};
+  const int f = a.fresh[s];
+  if (n.cached < 0 || f < 0 || n.cached > kSumCap || f > kSumCap - n.cached || n.shared < 0) {
+    n.bad = RH_STEP_BAD_LENGTH;
+  } else {
+    const int want = blocks_of(n.cached + f, a.block);
+    if (want > a.stride) n.bad = RH_STEP_TABLE_FULL;
+    n.need = {f, want - blocks_of(n.cached, a.block)};
+  }
+  return n;
+}
+
+template <int THREADS>
+__device__ __forceinline__ int bad_groups(const StepArgs& a) {
+  int bad = 0;
+  for (int g = threadIdx.x; g < a.n_groups; g += THREADS) {
+    const int first = a.group_seqs[2 * g], count = a.group_seqs[2 * g + 1];
+    if (first < 0 || count < 0 || first > a.n_seqs || count > a.n_seqs - first) bad = RH_STEP_BAD_LENGTH;
+  }
+  return bad;
+}
+
+__device__ __forceinline__ void put_totals(const StepArgs& a, Need all, int free, int status) {
+  a.row_off[a.n_seqs] = all.rows;
+  a.totals[0] = all.rows;
+  a.totals[1] = all.blocks;
+  a.totals[2] = free - all.blocks;
+  a.totals[3] = status;
 }
 
 // Row t: position p of sequence s in block `id`.
@@ -119,27 +158,17 @@ __global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) 
     const int s = base + threadIdx.x;
     mine = {0, 0};
     if (s < a.n_seqs) {
-      cached = a.cached[s];
-      shared = a.shared ? a.shared[s] : 0;
-      const int f = a.fresh[s];
-      if (cached < 0 || f < 0 || cached > kSumCap || f > kSumCap - cached || shared < 0) {
-        bad |= RH_STEP_BAD_LENGTH;
-      } else {
-        const int held = blocks_of(cached, a.block), want = blocks_of(cached + f, a.block);
-        if (want > a.stride) bad |= RH_STEP_TABLE_FULL;
-        mine = {f, want - held};
-        most = max(most, f);
-      }
+      const Length n = length_of(a, s);
+      cached = n.cached, shared = n.shared, mine = n.need;
+      bad |= n.bad;
+      most = max(most, mine.rows);
     }
     Need total;
     upto = block_scan<THREADS>(mine, waves[turn], &total);
     all.rows = capped_add(all.rows, total.rows);
     all.blocks = capped_add(all.blocks, total.blocks);
   }
-  for (int g = threadIdx.x; g < a.n_groups; g += THREADS) {
-    const int first = a.group_seqs[2 * g], count = a.group_seqs[2 * g + 1];
-    if (first < 0 || count < 0 || first > a.n_seqs || count > a.n_seqs - first) bad |= RH_STEP_BAD_LENGTH;
-  }
+  bad |= bad_groups<THREADS>(a);
   if (all.rows > a.max_rows) bad |= RH_STEP_ROWS_FULL;
   if (all.blocks > free) bad |= RH_STEP_NO_BLOCKS;
   if (a.n_seqs == 0) __syncthreads();  // (the scans' barriers follow s_bad's clearing)
@@ -202,13 +231,7 @@ __global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) 
       __syncthreads();
     }
   }
-  if (threadIdx.x == 0) {
-    a.row_off[a.n_seqs] = all.rows;
-    a.totals[0] = all.rows;
-    a.totals[1] = all.blocks;
-    a.totals[2] = free - all.blocks;
-    a.totals[3] = status;
-  }
+  if (threadIdx.x == 0) put_totals(a, all, free, status);
   if (a.n_groups || (ROWS && !own_rows)) __syncthreads();  // row_off and the tables are read below
   for (int g = threadIdx.x; g < a.n_groups; g += THREADS) {
     int4 v = {0, 0, 0, 0};
@@ -225,6 +248,86 @@ __global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) 
       for (int t = threadIdx.x; t < all.rows; t += THREADS) find_row(a, a.row_off, t);
     for (int t = all.rows + threadIdx.x; t < a.max_rows; t += THREADS) put_idle(a, t);
   }
+}
+
+// The whole step in many workgroups, each of which takes the sums for itself (they read the same few KB), keeps
+// every sequence's first row and first new id in LDS and then writes its rows; the first one writes what there is once
+// a sequence. A row whose block is new reads its id from the stack, so nobody waits for the tables.
+// Not where free_count is one of the totals, which the first may write before another has read it.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void step_wide_kernel(const StepArgs a) {
+  __shared__ Need waves[2][THREADS / 64];
+  __shared__ int s_bad, s_off[kRowOffsets], s_taken[kRowOffsets];
+  const int free = *a.free_count;
+  if (threadIdx.x == 0) s_bad = 0;
+  int bad = free < 0 ? RH_STEP_BAD_LENGTH : 0;
+  Need all = {0, 0};
+  for (int base = 0, turn = 0; base < a.n_seqs; base += THREADS, turn ^= 1) {
+    const int s = base + threadIdx.x;
+    Need mine = {0, 0};
+    if (s < a.n_seqs) {
+      const Length n = length_of(a, s);
+      bad |= n.bad;
+      mine = n.need;
+    }
+    Need total;
+    const Need upto = block_scan<THREADS>(mine, waves[turn], &total);
+    if (s < a.n_seqs) {
+      s_off[s] = capped_add(all.rows, upto.rows - mine.rows);
+      s_taken[s] = capped_add(all.blocks, upto.blocks - mine.blocks);
+    }
+    all.rows = capped_add(all.rows, total.rows);
+    all.blocks = capped_add(all.blocks, total.blocks);
+  }
+  bad |= bad_groups<THREADS>(a);
+  if (all.rows > a.max_rows) bad |= RH_STEP_ROWS_FULL;
+  if (all.blocks > free) bad |= RH_STEP_NO_BLOCKS;
+  if (a.n_seqs == 0) __syncthreads();  // (the scans' barriers follow s_bad's clearing)
+  if (bad) atomicOr(&s_bad, bad);
+  __syncthreads();
+  const int status = s_bad;
+  if (status) all = {0, 0};
+  const auto last_at = [&](const int* firsts, int k) {  // the last sequence that begins at or before k
+    int lo = 0, hi = a.n_seqs;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (firsts[mid] <= k)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo;
+  };
+  const int t = blockIdx.x * THREADS + threadIdx.x;
+  if (t < all.rows) {
+    const int s = last_at(s_off, t), cached = a.cached[s], p = cached + t - s_off[s], at = p / a.block, held = blocks_of(cached, a.block);
+    const int id = at < held ? a.tables[s * a.stride + at] : a.free_blocks[free - 1 - (s_taken[s] + at - held)];
+    put_row(a, t, s, p, id, a.shared ? a.shared[s] : 0);
+  } else if (t < a.max_rows) {
+    put_idle(a, t);
+  }
+  for (int k = t; k < all.blocks; k += gridDim.x * THREADS) {
+    const int s = last_at(s_taken, k);
+    a.tables[s * a.stride + blocks_of(a.cached[s], a.block) + k - s_taken[s]] = a.free_blocks[free - 1 - k];
+  }
+  if (blockIdx.x) return;
+  const auto off = [&](int s) { return status ? 0 : s < a.n_seqs ? s_off[s] : all.rows; };
+  for (int s = threadIdx.x; s < a.n_seqs; s += THREADS) {
+    a.row_off[s] = off(s);
+    a.last_row[s] = off(s + 1) > off(s) ? off(s + 1) - 1 : 0;
+    a.table_off[s] = s * a.stride;
+  }
+  for (int g = threadIdx.x; g < a.n_groups; g += THREADS) {
+    int4 v = {0, 0, 0, 0};
+    if (!status) {
+      const int first = a.group_seqs[2 * g], count = a.group_seqs[2 * g + 1];
+      v.x = off(first);
+      v.y = off(first + count) - v.x;
+      if (count) v.z = a.shared ? a.shared[first] : 0, v.w = first * a.stride;
+    }
+    a.groups[g] = v;
+  }
+  if (threadIdx.x == 0) put_totals(a, all, free, status);
 }
 
 __global__ __launch_bounds__(kRowThreads) void step_rows_kernel(const StepArgs a) {
@@ -646,7 +749,17 @@ int rh_step_tables(const int* cached, const int* fresh, const int* shared, int n
                    reinterpret_cast<int4*>(dec_meta), reinterpret_cast<int4*>(groups), totals};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(1), dim3(threads), 0, s, a); };
-  if (max_rows > kOneLaunch) {
+  const bool carried = free_count >= totals && free_count < totals + 4;
+  if (max_rows > kWideRows && n_seqs <= kRowOffsets && !carried) {
+    const auto wide = [&](auto kernel, int threads) {
+      hipLaunchKernelGGL(kernel, dim3((max_rows - 1) / threads + 1), dim3(threads), 0, s, a);
+    };
+    // Measured (us, 256 / 512 / 1024 threads): 64 sequences and 8 prompts of 512 4.8 / 4.8 / 5.3, 511 and 40 of 700 6.5 / 5.5 /
+    // 6.1, 2000 and 40 of 512 12.9 / 9.4 / 8.6, 4000 21.5 / 14.3 / 12.4.
+    RH_TRY_LAUNCH(n_seqs <= 256    ? wide(step_wide_kernel<256>, 256)
+                  : n_seqs <= 1024 ? wide(step_wide_kernel<512>, 512)
+                                   : wide(step_wide_kernel<1024>, 1024));
+  } else if (max_rows > kOneLaunch) {
     RH_TRY_LAUNCH(n_seqs <= 256 ? go(step_tables_kernel<256, false>, 256) : go(step_tables_kernel<1024, false>, 1024));
     RH_TRY_LAUNCH(hipLaunchKernelGGL(step_rows_kernel, dim3((max_rows + kRowThreads - 1) / kRowThreads), dim3(kRowThreads), 0, s, a));
   } else {

@@ -128,6 +128,18 @@ def test_step_tables_without_shared_and_with_carried_stack(torch_mod, dev):
 
 
 @gpu
+@pytest.mark.parametrize("seed,n,ctx,chunk,B,ng,carry", [
+    (30, 511, 200, 90, 16, 5, True), (31, 3, 5000, 9000, 16, 1, True), (32, 1500, 40, 5, 16, 3, True), (33, 200, 60, 30, 16, 2, True),
+    (34, 4096, 20, 3, 16, 4, False), (35, 4097, 20, 3, 16, 4, False), (36, 4097, 20, 30, 12, 2, True), (37, 257, 60, 4, 16, 1, False)])
+def test_step_tables_of_large_steps(torch_mod, dev, seed, n, ctx, chunk, B, ng, carry):
+    """More sequences than a workgroup keeps, and a stack count that lies in the totals."""
+    case = tables_case(seed, n, ctx, chunk, B, ng)
+    same(run_tables(torch_mod, dev, *case, carry=carry), tables_oracle(*case))
+    case = tables_case(seed, n, ctx, chunk, B, ng, short=3, waits=0.0)
+    same(run_tables(torch_mod, dev, *case, carry=carry), tables_oracle(*case))
+
+
+@gpu
 @pytest.mark.parametrize("change,status", [({"extra": -1}, ROWS_FULL), ({"short": 3}, NO_BLOCKS), ({"narrow": 3}, TABLE_FULL),
                                            ({"extra": -1, "short": 3}, ROWS_FULL | NO_BLOCKS)])
 @pytest.mark.parametrize("n", [40, 1500])
