@@ -38,6 +38,7 @@ constexpr int kStrip = 32;  // query rows of a wave: a strip
 constexpr int kStep = 32;   // keys of a wave's step
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
+constexpr int kLeast = kStep * kWaves;  // slices are multiples of as many keys
 constexpr int kFew = 16;    // query rows of a workgroup whose waves take keys of their own
 constexpr int kMerge = 8;   // slices whose values are loaded at once (attend_few)
 constexpr int kRing = 4;    // 32-key tiles of K and V in LDS, where strips share them
@@ -65,7 +66,8 @@ struct SharedArgs {
   int shared_slice, shared_parts, own_slice, own_parts, tiles, own_tiles;  // tiles: row tiles of a group, of a token
   int shared_units, shared_wgs, own_units;  // workgroups on prefixes come first
   int each, pieces;  // attend_few: tokens of a row tile, row tiles of a token (one of the two is 1)
-  Div by_tiles, by_own_tiles, by_shared_parts, by_own_parts, by_kv_heads, by_group;  // (by_group: rows of attend_few)
+  Div by_tiles, by_own_tiles, by_shared_parts, by_own_parts, by_kv_heads;
+  Div by_group, by_shared_slice, by_own_slice;  // of rows of attend_few, of 128 keys
   float scale_log2;
   int* counters;  // per token and kv head, counter_step apart: slices that have come (zero between calls)
   int counter_step;
@@ -74,9 +76,9 @@ struct SharedArgs {
   int64_t out_stride;
 };
 
-// Slices of `keys` keys where the launch has room for `most`; the last takes what is left.
-__device__ __forceinline__ int parts_of(int keys, int slice, int most) {
-  return keys <= 0 ? 0 : min(most, (keys + slice - 1) / slice);
+// Slices (of so many 128 keys) of `keys` keys where the launch has room for `most`; the last takes what is left.
+__device__ __forceinline__ int parts_of(int keys, const Div& slice, int most) {
+  return keys <= 0 ? 0 : min(most, slice(static_cast<int>((keys + (kLeast - 1u)) / kLeast) + static_cast<int>(slice.d) - 1));
 }
 
 __device__ __forceinline__ float row_max(float x) {
@@ -460,7 +462,7 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
       const int4 mt = a.meta[token0 + threadIdx.x];
       s_row[threadIdx.x] = mt.x;
       if (mt.y > 0)
-        slices = parts_of(mt.w, a.shared_slice, a.shared_parts) + parts_of(mt.y - max(mt.w, 0), a.own_slice, a.own_parts);
+        slices = parts_of(mt.w, a.by_shared_slice, a.shared_parts) + parts_of(mt.y - max(mt.w, 0), a.by_own_slice, a.own_parts);
     }
     const int lim = on ? min(m.y, end) : end;
     half8 qb[KH];
@@ -651,7 +653,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D > 64
     g.part = b - head * a.shared_parts;
     g.kvh = head - group * a.kv_heads;
     const int4 rec = a.groups[group];
-    const int parts = parts_of(rec.z, a.shared_slice, a.shared_parts);
+    const int parts = parts_of(rec.z, a.by_shared_slice, a.shared_parts);
     if (g.part >= parts) return;
     g.first = rec.x, g.members = rec.y, g.table = a.tables + rec.w;
     g.begin = g.part * a.shared_slice;
@@ -666,12 +668,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D > 64
     g.first = a.by_kv_heads(head), g.members = 1;
     g.kvh = head - g.first * a.kv_heads;
     const int4 m = a.meta[g.first];
-    const int from = max(m.w, 0), parts = parts_of(m.y - from, a.own_slice, a.own_parts);
+    const int from = max(m.w, 0), parts = parts_of(m.y - from, a.by_own_slice, a.own_parts);
     if (g.part >= parts) return;
     g.table = a.tables + m.z;
     g.begin = from + g.part * a.own_slice;
     g.end = g.part == parts - 1 ? m.y : g.begin + a.own_slice;
-    g.part += parts_of(m.w, a.shared_slice, a.shared_parts);
+    g.part += parts_of(m.w, a.by_shared_slice, a.shared_parts);
   }
   attend_few<D, DR, SCALAR, !ROWS>(a, g, smem);
 }
@@ -689,7 +691,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(const SharedArgs a) {
   const int4 m = a.meta[token];
   if (m.y <= 0) return;
   const int most = a.shared_parts + a.own_parts;
-  const int parts = parts_of(m.w, a.shared_slice, a.shared_parts) + parts_of(m.y - max(m.w, 0), a.own_slice, a.own_parts);
+  const int parts = parts_of(m.w, a.by_shared_slice, a.shared_parts) + parts_of(m.y - max(m.w, 0), a.by_own_slice, a.own_parts);
   const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + row * most;
   const float* o = a.part_o + row * most * D + d;
   float M = -INFINITY, L = 0.0f, O = 0.0f;
@@ -775,7 +777,7 @@ Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_o
   const double held = 256.0 * (head_dim > 64 ? 2 : 3);
   const double rate = 4e6;  // bytes a us
   const auto cut = [&](int64_t units, int keys, double step, int step_keys, double part, double beside, int* slice, int* parts) {
-    const int least = kStep * kWaves;
+    const int least = kLeast;
     double best = 0.0;
     *slice = least, *parts = 1;
     for (int want = 1; want <= 64; ++want) {
@@ -963,6 +965,8 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   a.by_shared_parts = div_by(p.shared_parts, wgs);
   a.by_own_parts = div_by(p.own_parts, wgs);
   a.by_kv_heads = div_by(kv_heads, wgs);
+  a.by_shared_slice = div_by(p.shared_slice / kLeast, (1 << 24) + p.shared_slice / kLeast);
+  a.by_own_slice = div_by(p.own_slice / kLeast, (1 << 24) + p.own_slice / kLeast);
   a.by_group = div_by(a.group, std::max(kFew, a.each * a.group) + 1);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (head_dim) {

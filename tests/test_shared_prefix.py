@@ -185,7 +185,7 @@ def test_large_scores_keep_their_order(torch_mod, dev):
 
 
 @gpu
-@pytest.mark.parametrize("hints", [(1, 0, 0), (1, 64, 16), (100, 5000, 5000), (0, 0, 0), (1000000, 64, 16)])
+@pytest.mark.parametrize("hints", [(1, 0, 0), (1, 64, 16), (100, 5000, 5000), (0, 0, 0), (1000000, 64, 16), (9, 3000000, 5000000)])
 def test_hints_choose_speed_not_results(torch_mod, dev, hints):
     check(torch_mod, dev, Case([(9, 640), (5, 1200)], [40, 300], 9, 3, 64, seed=6), hints=hints)
     check(torch_mod, dev, Case([(9, 640), (5, 1200)], [40, 300], 16, 4, 128, seed=6), hints=hints)
