@@ -768,40 +768,70 @@ Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_o
   const int64_t tiles = p.rows ? (rows + kWaves * kStrip - 1) / (kWaves * kStrip) : (static_cast<int64_t>(max_members) + each - 1) / each * pieces_of;
   p.tiles = static_cast<int>(std::min<int64_t>(std::max<int64_t>(1, tiles), 1 << 20));
   p.own_tiles = pieces_of;
-  // Slices of multiples of 128 keys, by what a launch of them takes (us, measured on MI355X): a start of
-  // 5, a step of 32 keys of 128 rows 1.05 at head size 128 and 0.5 below, of 128 own keys 1.5 and 0.8,
-  // in rounds of the workgroups that the card holds, and each slice's way through memory to its
-  // join. A prefix need not end before the own keys do: with 64 members on 16,384 keys and up to 1000 of
-  // their own (32/8 heads of 128) 8 / 12 / 16 / 32 slices take 79 / 69 / 72 / 86, with 45 members on 5
-  // prefixes of 1504 and up to 700 of their own 2 / 3 / 6 / 12 54 / 33 / 41 / 45.
-  const double held = 256.0 * (head_dim > 64 ? 2 : 3);
-  const double rate = 4e6;  // bytes a us
-  const auto cut = [&](int64_t units, int keys, double step, int step_keys, double part, double beside, int* slice, int* parts) {
-    const int least = kLeast;
+  const double held = 256.0 * (head_dim > 64 ? 2 : 3);  // workgroups that the card holds
+  const int64_t own_units = static_cast<int64_t>(n_dec) * kv_heads * p.own_tiles;
+  const int64_t shared_units = static_cast<int64_t>(n_groups) * kv_heads * p.tiles;
+  const auto slice_of = [](int keys, int want) {
+    return static_cast<int>((static_cast<int64_t>(keys) + static_cast<int64_t>(want) * kLeast - 1) / (static_cast<int64_t>(want) * kLeast)) * kLeast;
+  };
+  const auto put = [&](int keys, int size, int* slice, int* parts) {
+    *slice = std::max(size, kLeast), *parts = size < kLeast ? 1 : (keys + size - 1) / size;
+  };
+  if (p.rows) {
+    // Both kinds' slices together, by what the call then takes (us): a start and the steps of either; all of
+    // them in the card's places, and half a last one; no less than their bytes; each slice's way through memory to
+    // its join. (Own lengths spread below the largest.) Constants from timings of every cut of 30 shapes; the cut that the
+    // rule takes is 1.5% from the best on average, 8% at worst. Two rules, each for its own kind alone, took 8%: 4 x 8 members
+    // on 2000 keys with 300 of their own (32/8 heads of 128), 16 slices and 2 own 32 us, 8 and 1 23; 64 on 16,384
+    // with 1000, 13 and 1 64 us, 32 and 1 86.
+    const double step = head_dim > 64 ? 0.75 : 0.6, own_step = head_dim > 64 ? 1.2 : 0.75, spread = 0.72;
+    const double bytes = (static_cast<double>(n_groups) * max_shared + spread * n_dec * max_own) * kv_heads * head_dim * 4;
+    const double part = static_cast<double>(n_dec) * heads * head_dim * 8 / 1.9e6;
     double best = 0.0;
-    *slice = least, *parts = 1;
+    for (const int want : {1, 2, 3, 4, 5, 6, 8, 10, 11, 13, 16, 19, 22, 26, 32, 43, 64}) {
+      const int size = slice_of(max_shared, want), n = size < kLeast ? 1 : (max_shared + size - 1) / size;
+      const double time = 4.8 + step * size / kStep;
+      for (const int own_want : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+        const int own_size = slice_of(max_own, own_want), own_n = own_size < kLeast ? 1 : (max_own + own_size - 1) / own_size;
+        const double own_time = 5.2 + own_step * std::min(own_size, max_own) / kLeast;
+        const double own_mean = 5.2 + own_step * std::min<double>(own_size, spread * max_own) / kLeast;
+        const double places = (static_cast<double>(shared_units) * n + static_cast<double>(own_units) * own_n) / held;
+        const double work = (shared_units * n * time + 0.57 * own_units * own_n * own_mean) / held + (places > 1.0 ? 0.5 * own_time : 0.0);
+        const double cost = std::max({time, own_time, work, bytes / 6.6e6}) + part * (n + own_n);
+        if (best == 0.0 || cost < best) {
+          best = cost;
+          put(max_shared, size, &p.shared_slice, &p.shared_parts);
+          put(max_own, own_size, &p.own_slice, &p.own_parts);
+        }
+        if (own_size <= kLeast) break;
+      }
+      if (size <= kLeast) break;
+    }
+    return p;
+  }
+  // Few rows: each kind by its own time, and what its slices cost the workgroup that joins them (us: a start of 5, a step of
+  // 128 keys 1.5 at head size 128 and 0.8 below, in rounds of the card's places).
+  const auto cut = [&](int64_t units, int keys, int64_t rows_joined, int* slice, int* parts) {
+    const double part = 0.09 * std::max(1.0, std::min<int64_t>(rows_joined, kFew) * head_dim / 256.0);
+    double best = 0.0;
+    put(keys, 0, slice, parts);
     for (int want = 1; want <= 64; ++want) {
-      const int size = static_cast<int>((static_cast<int64_t>(keys) + static_cast<int64_t>(want) * least - 1) / (static_cast<int64_t>(want) * least)) * least;
-      if (size < least) break;
+      const int size = slice_of(keys, want);
+      if (size < kLeast) break;
       const int n = (keys + size - 1) / size;
       const double rounds = static_cast<double>(units) * n / held;  // a last one is rarely full
-      const double time = (5.0 + step * size / step_keys) * (rounds <= 1.0 ? 1.0 : rounds + 0.5);
-      const double cost = std::max(time, beside) + part * n;
+      const double cost = (5.0 + (head_dim > 64 ? 1.5 : 0.8) * size / kLeast) * (rounds <= 1.0 ? 1.0 : rounds + 0.5) + part * n;
       if (want == 1 || cost < best) best = cost, *slice = size, *parts = n;
-      if (size == least) break;
+      if (size == kLeast) break;
     }
   };
-  const double own_step = head_dim > 64 ? 1.5 : 0.8;
-  const auto joined = [&](int64_t n) { return 0.09 * std::max(1.0, std::min<int64_t>(n, kFew) * head_dim / 256.0); };
-  // (Lengths spread below the largest: two thirds of it on average.)
-  const double own_time = 4.0 + 0.65 * n_dec * kv_heads * static_cast<double>(max_own) * head_dim * 4 / rate;
-  cut(static_cast<int64_t>(n_dec) * kv_heads * p.own_tiles, max_own, own_step, kStep * kWaves, joined(group), 0.0, &p.own_slice, &p.own_parts);
-  if (p.rows)
-    cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, max_shared, head_dim > 64 ? 1.05 : 0.5, kStep,
-        static_cast<double>(n_dec) * heads * head_dim * 8 / rate, own_time, &p.shared_slice, &p.shared_parts);
-  else
-    cut(static_cast<int64_t>(n_groups) * kv_heads * p.tiles, max_shared, own_step, kStep * kWaves, joined(rows), 0.0, &p.shared_slice, &p.shared_parts);
+  cut(own_units, max_own, group, &p.own_slice, &p.own_parts);
+  cut(shared_units, max_shared, rows, &p.shared_slice, &p.shared_parts);
   return p;
+}
+
+size_t bytes_of(const Plan& p, int n_dec, int heads, int head_dim) {
+  return kCounters * 4 + static_cast<size_t>(n_dec) * heads * (p.shared_parts + p.own_parts) * (head_dim + 2) * 4;
 }
 
 }  // namespace
@@ -887,12 +917,10 @@ extern "C" size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_me
   if (n_dec <= 0 || n_groups < 0 || max_members < 0 || max_shared < 0 || max_own < 0 || max_shared > kMostKeys || max_own > kMostKeys || kv_heads <= 0 || heads <= 0 ||
       heads % kv_heads || head_dim <= 0)
     return 0;
-  size_t parts = 0;  // enough for any block size
-  for (const int block : {1, 16}) {
-    const Plan p = plan_of(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim, block);
-    parts = std::max<size_t>(parts, p.shared_parts + p.own_parts);
-  }
-  return kCounters * 4 + static_cast<size_t>(n_dec) * heads * parts * (head_dim + 2) * 4;
+  size_t most = 0;  // enough for any block size
+  for (const int block : {1, 16})
+    most = std::max(most, bytes_of(plan_of(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim, block), n_dec, heads, head_dim));
+  return most;
 }
 
 extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, const void* kpool, const void* vpool,
@@ -917,10 +945,10 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   RH_REQUIRE((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kpool) | reinterpret_cast<uintptr_t>(vpool) |
               reinterpret_cast<uintptr_t>(dec_meta) | reinterpret_cast<uintptr_t>(groups)) % 16 == 0,
              "shared prefix attention: q, the pools, dec_meta and groups must be 16-byte aligned");
-  const size_t need = rh_shared_prefix_workspace(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim);
-  RH_REQUIRE(workspace_bytes >= need && (!need || (workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0)),
-             "shared prefix attention: needs a 16-byte aligned workspace of rh_shared_prefix_workspace bytes");
   const Plan p = plan_of(n_dec, n_groups, max_members, max_shared, max_own, heads, kv_heads, head_dim, block_size);
+  const size_t need = bytes_of(p, n_dec, heads, head_dim);
+  RH_REQUIRE(workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(workspace) % 16 == 0,
+             "shared prefix attention: needs a 16-byte aligned workspace of rh_shared_prefix_workspace bytes");
   SharedArgs a{};
   a.q = static_cast<const half_t*>(q);
   a.q_stride = q_row_stride;
