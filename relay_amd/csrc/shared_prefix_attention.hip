@@ -843,10 +843,11 @@ extern "C" int rh_shared_prefix_pays(int n_dec, int max_shared, int max_own, int
   if (n_dec <= 0 || max_shared <= 0 || max_own < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
   // What each token reads by itself, of which all but one reading of a prefix come from the caches: up to 100
   // MB the decode kernel's one launch and smaller steps win. Measured (us, decode / shared; members x shared +
-  // own): 32/8 heads of 128, 4 x 4096 + 300 (70 MB) 15.1 / 18.6, 16 x 1024 + 200 (76) 14.3 / 16.2, 32 x 1024 + 300
-  // (160) 28 / 22, 32 x 4096 + 300 (562) 58 / 26; 32/4 of 64, 32 x 1024 + 300 (40) 10.3 / 13.6, 32 x 4096 + 300 (141)
-  // 18.4 / 18.2, 64 x 2048 + 500 (156) 21 / 18; 9/3 of 64, 64 x 512 + 100 (28) 11.7 / 11.8, 32 x 4096 + 300 (106) 21 / 16.
-  // 16 query heads of 128 a kv head merge slowly there: 16/1, 2 x 4096 + 100 23 / 16, 64 x 512 + 100 13.5 / 15.5.
+  // own): 32/8 heads of 128, 4 x 4096 + 304 (70 MB) 15.2 / 19.0, 16 x 1024 + 200 (76) 14.3 / 15.5, 24 x 1024 + 100
+  // (107) 21 / 16, 32 x 1024 + 300 (160) 28 / 20, 32 x 4096 + 300 (562) 58 / 25; 32/4 of 64, 32 x 1024 + 300 (40) 10.3 / 13.1, 8
+  // groups of 4 x 3008 + 300 (105) 17.6 / 16.9, 32 x 4096 + 300 (141) 18.4 / 17.6, 64 x 2048 + 500 (156) 21 / 18; 9/3 of 64, 64 x
+  // 512 + 100 (28) 11.6 / 11.5, 32 x 4096 + 300 (105) 21 / 15.
+  // 16 query heads of 128 a kv head merge slowly there: 16/1, 2 x 4096 + 100 23 / 16, 64 x 512 + 100 13.6 / 15.3.
   const double alone = static_cast<double>(n_dec) * kv_heads * head_dim * 4 * (max_shared + 0.65 * max_own);
   return alone > 100e6 || static_cast<int64_t>(heads / kv_heads) * head_dim > 1024;
 }
