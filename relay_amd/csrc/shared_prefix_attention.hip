@@ -11,14 +11,14 @@
 //
 //  - many rows (prefixes of more than 16 rows or 1024 keys, or of more than 12 rows of 128): 128 rows, 32 a
 //    wave, on tiles of K and V that the waves share in LDS (attend_rows). 64 x 4 rows on 16,384 keys of
-//    8 heads of 128 (17 GFLOP, 67 MB) take 39 us, the join of their 32 slices 10. Bound by the chain of a
+//    8 heads of 128 (17 GFLOP, 67 MB) take 40 us, the join of their 16 slices 8. Bound by the chain of a
 //    step (LDS reads, products, weights: no one of them taken out made it faster by over a tenth); a
-//    ring of five tiles, which leaves a CU one workgroup, takes 5-10% longer.
+//    ring of five tiles takes 5-10% longer.
 //  - few rows (own keys, short prefixes): 16 rows, the waves on keys of their own, K straight into MFMA
 //    operands (attend_few). Bound by memory: 64 x 1000 own keys, 8 kv heads of 128 (ragged, 164 MB) 34 us.
 //
 // One launch does both, prefixes first: the prefix's products run beside the own keys' loads. 64 members on
-// 16,384 keys with up to 1000 of their own (231 MB, 18 GFLOP) take 57 us, the join 6. Prefix tiles staged
+// 16,384 keys with up to 1000 of their own (231 MB, 18 GFLOP) take 59 us, the join 6. Prefix tiles staged
 // through registers, whose reloads from scratch waited for every load in flight, took 107 in all, and
 // workgroups of eight waves that do not share their tiles 244.
 #include <algorithm>
