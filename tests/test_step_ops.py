@@ -128,6 +128,18 @@ def test_step_tables_without_shared_and_with_carried_stack(torch_mod, dev):
 
 
 @gpu
+@pytest.mark.parametrize("max_rows", [512, 513, 5000])
+def test_step_tables_of_idle_rows(torch_mod, dev, max_rows):
+    got = run_tables(torch_mod, dev, np.zeros(0, int), np.zeros(0, int), np.zeros(0, int), [], 16, np.zeros((0, 4), int), np.arange(3), max_rows)
+    assert (got["slot"] == -1).all() and (got["meta"][:, 1] == 0).all() and got["totals"].tolist() == [0, 0, 3, 0] and got["row_off"].tolist() == [0]
+    c = list(tables_case(24, 6, 60, 1, 16, 2))
+    c[-1] = max_rows
+    same(run_tables(torch_mod, dev, *c), tables_oracle(*c))
+    c[1] = np.zeros(6, int)
+    same(run_tables(torch_mod, dev, *c), tables_oracle(*c))
+
+
+@gpu
 @pytest.mark.parametrize("seed,n,ctx,chunk,B,ng,carry", [
     (30, 511, 200, 90, 16, 5, True), (31, 3, 5000, 9000, 16, 1, True), (32, 1500, 40, 5, 16, 3, True), (33, 200, 60, 30, 16, 2, True),
     (34, 4096, 20, 3, 16, 4, False), (35, 4097, 20, 3, 16, 4, False), (36, 4097, 20, 30, 12, 2, True), (37, 257, 60, 4, 16, 1, False)])
