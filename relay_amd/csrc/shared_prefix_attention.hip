@@ -43,16 +43,19 @@ constexpr int kFew = 16;    // query rows of a workgroup whose waves take keys o
 constexpr int kMerge = 8;   // slices whose values are loaded at once (attend_few)
 constexpr int kRing = 4;    // 32-key tiles of K and V in LDS, where strips share them
 
-// n / d for 0 <= n < limit by one multiplication (m = ceil(2^32 / d) is exact while n * d < 2^32; else m is 0
-// and the division is made): an integer division is some 40 instructions, and a workgroup's place takes six.
+// n / d for 0 <= n < 2^31 by one multiplication: with d <= 2^shift and m = ceil(2^(31 + shift) / d), n * m is
+// above n * 2^(31 + shift) / d by less than n * d / d < 2^31 parts of it in 2^(31 + shift), too little to reach the next
+// whole number. (An integer division is some 40 instructions, and a workgroup's place takes six.)
 struct Div {
-  unsigned d, m;
+  unsigned d, m, shift;
   __device__ __forceinline__ int operator()(int n) const {
-    return d == 1 ? n : m ? static_cast<int>(__umulhi(static_cast<unsigned>(n), m)) : static_cast<int>(static_cast<unsigned>(n) / d);
+    return static_cast<int>(__umulhi(2u * static_cast<unsigned>(n), m) >> shift);
   }
 };
-Div div_by(int d, int64_t limit) {
-  return {static_cast<unsigned>(d), d > 1 && limit * d < (int64_t{1} << 32) ? static_cast<unsigned>(((int64_t{1} << 32) + d - 1) / d) : 0u};
+Div div_by(int d) {
+  unsigned shift = 0;
+  while ((int64_t{1} << shift) < d) ++shift;
+  return {static_cast<unsigned>(d), static_cast<unsigned>(((uint64_t{1} << (31 + shift)) + d - 1) / d), shift};
 }
 
 struct SharedArgs {
@@ -989,14 +992,14 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
   a.shared_wgs = static_cast<int>(shared_wgs);
   a.each = std::max(1, kFew / a.group);
   a.pieces = (a.group + kFew - 1) / kFew;
-  a.by_tiles = div_by(p.tiles, wgs);
-  a.by_own_tiles = div_by(p.own_tiles, wgs);
-  a.by_shared_parts = div_by(p.shared_parts, wgs);
-  a.by_own_parts = div_by(p.own_parts, wgs);
-  a.by_kv_heads = div_by(kv_heads, wgs);
-  a.by_shared_slice = div_by(p.shared_slice / kLeast, (1 << 24) + p.shared_slice / kLeast);
-  a.by_own_slice = div_by(p.own_slice / kLeast, (1 << 24) + p.own_slice / kLeast);
-  a.by_group = div_by(a.group, std::max(kFew, a.each * a.group) + 1);
+  a.by_tiles = div_by(p.tiles);
+  a.by_own_tiles = div_by(p.own_tiles);
+  a.by_shared_parts = div_by(p.shared_parts);
+  a.by_own_parts = div_by(p.own_parts);
+  a.by_kv_heads = div_by(kv_heads);
+  a.by_shared_slice = div_by(p.shared_slice / kLeast);
+  a.by_own_slice = div_by(p.own_slice / kLeast);
+  a.by_group = div_by(a.group);
   hipStream_t s = static_cast<hipStream_t>(stream);
   switch (head_dim) {
     case 16: if (int rc = launch<32, 16>(a, p.rows, wgs, s)) return rc; break;
