@@ -125,6 +125,23 @@ __device__ __forceinline__ float coherent_load(const float* p) {
   return __hip_atomic_load(const_cast<float*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// ---- division by a number that the host knows --------------------------------------------
+
+// n / d for 0 <= n < 2^31 by one multiplication: with d <= 2^shift and m = ceil(2^(31 + shift) / d), n * m is
+// above n * 2^(31 + shift) / d by less than n * d / d < 2^31 parts of it in 2^(31 + shift), too little to reach the next
+// whole number. (An integer division is some 40 instructions.)
+struct Div {
+  unsigned d, m, shift;
+  __device__ __forceinline__ int operator()(int n) const {
+    return static_cast<int>(__umulhi(2u * static_cast<unsigned>(n), m) >> shift);
+  }
+};
+inline Div div_by(int d) {
+  unsigned shift = 0;
+  while ((int64_t{1} << shift) < d) ++shift;
+  return {static_cast<unsigned>(d), static_cast<unsigned>(((uint64_t{1} << (31 + shift)) + d - 1) / d), shift};
+}
+
 // ---- the raw partial planes of a split product -------------------------------------------
 
 constexpr int kMaxMergeSplit = 8;

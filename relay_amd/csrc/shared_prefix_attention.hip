@@ -43,21 +43,6 @@ constexpr int kFew = 16;    // query rows of a workgroup whose waves take keys o
 constexpr int kMerge = 8;   // slices whose values are loaded at once (attend_few)
 constexpr int kRing = 4;    // 32-key tiles of K and V in LDS, where strips share them
 
-// n / d for 0 <= n < 2^31 by one multiplication: with d <= 2^shift and m = ceil(2^(31 + shift) / d), n * m is
-// above n * 2^(31 + shift) / d by less than n * d / d < 2^31 parts of it in 2^(31 + shift), too little to reach the next
-// whole number. (An integer division is some 40 instructions, and a workgroup's place takes six.)
-struct Div {
-  unsigned d, m, shift;
-  __device__ __forceinline__ int operator()(int n) const {
-    return static_cast<int>(__umulhi(2u * static_cast<unsigned>(n), m) >> shift);
-  }
-};
-Div div_by(int d) {
-  unsigned shift = 0;
-  while ((int64_t{1} << shift) < d) ++shift;
-  return {static_cast<unsigned>(d), static_cast<unsigned>(((uint64_t{1} << (31 + shift)) + d - 1) / d), shift};
-}
-
 struct SharedArgs {
   const half_t* q;
   int64_t q_stride;

@@ -35,6 +35,7 @@ constexpr int kRowOffsets = 4096;        // sequences whose first rows a workgro
 struct StepArgs {
   const int *cached, *fresh, *shared, *group_seqs;
   int n_seqs, n_groups, block;
+  Div by_block;
   int* tables;
   int stride;
   const int *free_blocks, *free_count;
@@ -45,9 +46,7 @@ struct StepArgs {
 };
 
 __device__ __forceinline__ int capped_add(int a, int b) { return min(a + b, kSumCap); }
-__device__ __forceinline__ int blocks_of(int keys, int block) {
-  return static_cast<int>((static_cast<unsigned>(keys) + static_cast<unsigned>(block) - 1u) / static_cast<unsigned>(block));
-}
+__device__ __forceinline__ int blocks_of(int keys, const Div& block) { return block(keys + static_cast<int>(block.d) - 1); }
 
 struct Need {
   int rows, blocks;
@@ -88,9 +87,9 @@ __device__ __forceinline__ Length length_of(const StepArgs& a, int s) {
   if (n.cached < 0 || f < 0 || n.cached > kSumCap || f > kSumCap - n.cached || n.shared < 0) {
     n.bad = RH_STEP_BAD_LENGTH;
   } else {
-    const int want = blocks_of(n.cached + f, a.block);
+    const int want = blocks_of(n.cached + f, a.by_block);
     if (want > a.stride) n.bad = RH_STEP_TABLE_FULL;
-    n.need = {f, want - blocks_of(n.cached, a.block)};
+    n.need = {f, want - blocks_of(n.cached, a.by_block)};
   }
   return n;
 }
@@ -117,7 +116,7 @@ __device__ __forceinline__ void put_totals(const StepArgs& a, Need all, int free
 __device__ __forceinline__ void put_row(const StepArgs& a, int t, int s, int p, int id, int shared) {
   a.pos[t] = p;
   a.seq[t] = s;
-  a.slot[t] = id * a.block + p % a.block;
+  a.slot[t] = id * a.block + p - a.by_block(p) * a.block;
   a.meta[t] = int4{t, p + 1, s * a.stride, shared};
 }
 
@@ -140,7 +139,7 @@ __device__ __forceinline__ void find_row(const StepArgs& a, const int* row_off, 
       hi = mid;
   }
   const int p = a.cached[lo] + t - row_off[lo];
-  put_row(a, t, lo, p, a.tables[lo * a.stride + p / a.block], a.shared ? a.shared[lo] : 0);
+  put_row(a, t, lo, p, a.tables[lo * a.stride + a.by_block(p)], a.shared ? a.shared[lo] : 0);
 }
 
 // ROWS: the rows too.
@@ -187,7 +186,7 @@ __global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) 
       if (s < a.n_seqs && !status) {
         cached = a.cached[s];
         shared = a.shared ? a.shared[s] : 0;
-        mine = {a.fresh[s], blocks_of(cached + a.fresh[s], a.block) - blocks_of(cached, a.block)};
+        mine = {a.fresh[s], blocks_of(cached + a.fresh[s], a.by_block) - blocks_of(cached, a.by_block)};
       }
       Need total;
       upto = block_scan<THREADS>(mine, waves[turn], &total);
@@ -200,7 +199,7 @@ __global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) 
       a.row_off[s] = row;
       a.last_row[s] = mine.rows ? upto.rows - 1 : 0;
       a.table_off[s] = s * a.stride;
-      const int held = blocks_of(cached, a.block);
+      const int held = blocks_of(cached, a.by_block);
       int* const table = a.tables + static_cast<int64_t>(s) * a.stride;
       s_taken[threadIdx.x] = first;
       s_held[threadIdx.x] = held;
@@ -208,7 +207,7 @@ __global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) 
         for (int j = 0; j < mine.blocks; ++j) table[held + j] = a.free_blocks[free - 1 - (first + j)];
       if (own_rows) {
         for (int j = 0; j < mine.rows; ++j) {
-          const int at = (cached + j) / a.block;
+          const int at = a.by_block(cached + j);
           put_row(a, row + j, s, cached + j, at < held ? table[at] : a.free_blocks[free - 1 - (first + at - held)], shared);
         }
       }
@@ -300,7 +299,7 @@ __global__ __launch_bounds__(THREADS) void step_wide_kernel(const StepArgs a) {
   };
   const int t = blockIdx.x * THREADS + threadIdx.x;
   if (t < all.rows) {
-    const int s = last_at(s_off, t), cached = a.cached[s], p = cached + t - s_off[s], at = p / a.block, held = blocks_of(cached, a.block);
+    const int s = last_at(s_off, t), cached = a.cached[s], p = cached + t - s_off[s], at = a.by_block(p), held = blocks_of(cached, a.by_block);
     const int id = at < held ? a.tables[s * a.stride + at] : a.free_blocks[free - 1 - (s_taken[s] + at - held)];
     put_row(a, t, s, p, id, a.shared ? a.shared[s] : 0);
   } else if (t < a.max_rows) {
@@ -308,7 +307,7 @@ __global__ __launch_bounds__(THREADS) void step_wide_kernel(const StepArgs a) {
   }
   for (int k = t; k < all.blocks; k += gridDim.x * THREADS) {
     const int s = last_at(s_taken, k);
-    a.tables[s * a.stride + blocks_of(a.cached[s], a.block) + k - s_taken[s]] = a.free_blocks[free - 1 - k];
+    a.tables[s * a.stride + blocks_of(a.cached[s], a.by_block) + k - s_taken[s]] = a.free_blocks[free - 1 - k];
   }
   if (blockIdx.x) return;
   const auto off = [&](int s) { return status ? 0 : s < a.n_seqs ? s_off[s] : all.rows; };
@@ -370,23 +369,25 @@ struct QkArgs {
   half_t *kpool, *vpool, *q_out;
   float q_scale;
   int heads, kv_heads, D, block;
+  Div by_block, by_sets;  // by_sets: sets of heads a token
 };
 
 // PLAIN: one plane and no scale, without the branches of up to 8 (2047 rows of 32/4 heads of 64 11.0 / 10.4 us).
 template <int LANES, int HEADS, bool PLAIN>
-__global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a, int sets) {
+__global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a) {
   constexpr int PER = kWave / LANES;  // heads of a set
   // The arguments at once: the compiler loads them where they are used, one wait after another (2047 rows of 32/4
   // heads of 64 10.4 -> 9.4 us; the tables' and the logits' kernels gain nothing by it).
   asm volatile("" : : "s"(a.qkv), "s"(a.planes), "s"(a.scale), "s"(a.T), "s"(a.bias), "s"(a.q_norm), "s"(a.k_norm), "s"(a.eps), "s"(a.inv_freq),
                "s"(a.pos), "s"(a.slot), "s"(a.kpool), "s"(a.vpool), "s"(a.q_out), "s"(a.q_scale), "s"(a.heads), "s"(a.kv_heads), "s"(a.D),
-               "s"(a.block));
+               "s"(a.block), "s"(a.by_block.m), "s"(a.by_sets.m));
   const int unit = blockIdx.x * (kThreads / kWave) + (threadIdx.x >> 6);  // (token, HEADS sets)
-  const int t = unit / sets, h0 = unit % sets * (PER * HEADS) + (threadIdx.x & 63) / LANES, i = 4 * (threadIdx.x % LANES);
+  const int t = a.by_sets(unit), h0 = (unit - t * static_cast<int>(a.by_sets.d)) * (PER * HEADS) + (threadIdx.x & 63) / LANES, i = 4 * (threadIdx.x % LANES);
   if (t >= a.T) return;
   const int slot = a.slot[t];
   const double p = a.pos[t];
   if (slot < 0) return;  // an idle row
+  const int block = a.by_block(slot);
   const int half = a.D / 2, total = a.heads + 2 * a.kv_heads;
   const int64_t width = static_cast<int64_t>(total) * a.D, plane = a.T * width;
   float x[HEADS][4], y[HEADS][4];
@@ -444,7 +445,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a, int s
       f = a.q_scale;
     } else {
       dst = (turned ? a.kpool : a.vpool) +
-            kv_row_offset(slot / a.block, a.kv_heads, (h - a.heads) % a.kv_heads, a.block, slot % a.block, a.D) + i;
+            kv_row_offset(block, a.kv_heads, h - a.heads - (turned ? 0 : a.kv_heads), a.block, slot - block * a.block, a.D) + i;
     }
     half4 ox, oy;
 #pragma unroll
@@ -749,7 +750,7 @@ int rh_step_tables(const int* cached, const int* fresh, const int* shared, int n
              "step tables: missing pointer");
   RH_REQUIRE((reinterpret_cast<uintptr_t>(dec_meta) | reinterpret_cast<uintptr_t>(groups)) % 16 == 0,
              "step tables: dec_meta and groups must be 16-byte aligned");
-  const StepArgs a{cached, fresh, shared, group_seqs, n_seqs, n_groups, block_size, tables, table_stride, free_blocks,
+  const StepArgs a{cached, fresh, shared, group_seqs, n_seqs, n_groups, block_size, div_by(block_size), tables, table_stride, free_blocks,
                    free_count, max_rows, row_off, last_row, table_off, pos, seq, slot,
                    reinterpret_cast<int4*>(dec_meta), reinterpret_cast<int4*>(groups), totals};
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -787,7 +788,7 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
                   reinterpret_cast<uintptr_t>(vpool)) % 8 == 0,
              "qk_norm: qkv must be 16-byte aligned, q_out and the pools 8-byte");
   const QkArgs a{qkv, planes, scale, T, bias, q_norm, k_norm, eps, inv_freq, pos, slot, static_cast<half_t*>(kpool),
-                 static_cast<half_t*>(vpool), static_cast<half_t*>(q_out), q_scale, heads, kv_heads, head_dim, block_size};
+                 static_cast<half_t*>(vpool), static_cast<half_t*>(q_out), q_scale, heads, kv_heads, head_dim, block_size, div_by(block_size), {}};
   const int total = heads + 2 * kv_heads;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const auto of_lanes = [&](auto lanes) -> int {
@@ -795,7 +796,9 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
     const auto go = [&](auto kernel, int per_wave) -> int {
       const int64_t sets = (total + per_wave - 1) / per_wave, wgs = (T * sets + kThreads / kWave - 1) / (kThreads / kWave);
       RH_REQUIRE(T * sets + kThreads < (int64_t{1} << 31), "qk_norm: too many rows");
-      RH_TRY_LAUNCH(hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(kThreads), 0, s, a, static_cast<int>(sets)));
+      QkArgs b = a;
+      b.by_sets = div_by(static_cast<int>(sets));
+      RH_TRY_LAUNCH(hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(kThreads), 0, s, b));
       return 0;
     };
     constexpr int PER = kWave / LANES;
