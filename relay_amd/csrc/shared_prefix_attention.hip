@@ -18,7 +18,7 @@
 //    operands (attend_few). Bound by memory: 64 x 1000 own keys, 8 kv heads of 128 (ragged, 164 MB) 34 us.
 //
 // One launch does both, prefixes first: the prefix's products run beside the own keys' loads. 64 members on
-// 16,384 keys with up to 1000 of their own (231 MB, 18 GFLOP) take 59 us, the join 6. Prefix tiles staged
+// 16,384 keys with up to 1000 of their own (231 MB, 18 GFLOP) take 58 us, the join 5.5. Prefix tiles staged
 // through registers, whose reloads from scratch waited for every load in flight, took 107 in all, and
 // workgroups of eight waves that do not share their tiles 244.
 #include <algorithm>

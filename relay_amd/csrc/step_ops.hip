@@ -20,7 +20,7 @@ namespace {
 // row_off[s + 1] - 1: two exclusive sums over the sequences, a chain of dependent steps that bounds the call.
 // Up to kWideRows rows one workgroup takes them, a sequence a thread (more in several turns); where no
 // sequence adds more than kOwnRows tokens, as in decoding, its thread writes its rows too, from what it
-// has in registers (48 decoding sequences 3.9 us, with a search for each row's sequence 6.3). Larger steps take
+// has in registers (48 decoding sequences 3.9 us, with a search for each row's sequence 6). Larger steps take
 // many workgroups that all make the sums (step_wide_kernel; 511 sequences of which 40 add a prompt, 26,500
 // rows, 5.5 us), unless the stack's count lies in the totals: then one workgroup makes them, with the rows in a
 // second launch past kOneLaunch of them (9.4 us; in one workgroup 58).
@@ -372,7 +372,7 @@ struct QkArgs {
   Div by_block, by_sets;  // by_sets: sets of heads a token
 };
 
-// PLAIN: one plane and no scale, without the branches of up to 8 (2047 rows of 32/4 heads of 64 11.0 / 10.4 us).
+// PLAIN: one plane and no scale, without the branches of up to 8 (2047 rows of 32/4 heads of 64 9.6 us, with them 10.9).
 template <int LANES, int HEADS, bool PLAIN>
 __global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a) {
   constexpr int PER = kWave / LANES;  // heads of a set
@@ -761,7 +761,7 @@ int rh_step_tables(const int* cached, const int* fresh, const int* shared, int n
       hipLaunchKernelGGL(kernel, dim3((max_rows - 1) / threads + 1), dim3(threads), 0, s, a);
     };
     // Measured (us, 256 / 512 / 1024 threads): 64 sequences and 8 prompts of 512 4.8 / 4.8 / 5.3, 511 and 40 of 700 6.5 / 5.5 /
-    // 6.1, 2000 and 40 of 512 12.9 / 9.4 / 8.6, 4000 21.5 / 14.3 / 12.4.
+    // 6.1, 2000 and 40 of 512 12.9 / 9.4 / 8.6 (now 8.2), 4000 21.5 / 14.3 / 12.4 (11.7).
     RH_TRY_LAUNCH(n_seqs <= 256    ? wide(step_wide_kernel<256>, 256)
                   : n_seqs <= 1024 ? wide(step_wide_kernel<512>, 512)
                                    : wide(step_wide_kernel<1024>, 1024));
@@ -803,8 +803,8 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
     };
     constexpr int PER = kWave / LANES;
     // Two sets of heads a wave once that leaves enough waves. Measured (us, one / two; bound by latency
-    // below, by memory above): 48 rows of 32/4 heads of 64 3.4 / 3.6, 256 3.7 / 3.8, 512 4.4 / 4.3, 2047 11.5 /
-    // 10.4 (floor 6.1), 4096 of 32/8 heads of 128 39 / 36 (29); three to five sets are level.
+    // below, by memory above): 48 rows of 32/4 heads of 64 3.2 / 3.6, 256 3.6 / 3.7, 512 4.3 / 4.3, 2047 10.3 /
+    // 9.6 (floor 6.1), 4096 of 32/8 heads of 128 37 / 33 (29); three to five sets are level.
     const bool many = static_cast<int64_t>(T) * total * LANES >= 150000;
     if (planes == 1 && !scale) return many ? go(qk_norm_kernel<LANES, 2, true>, 2 * PER) : go(qk_norm_kernel<LANES, 1, true>, PER);
     return many ? go(qk_norm_kernel<LANES, 2, false>, 2 * PER) : go(qk_norm_kernel<LANES, 1, false>, PER);
