@@ -156,6 +156,17 @@ __device__ __forceinline__ void mask_keys(float16v& s, int key0, int lo, int lim
   }
 }
 
+// One fma a score, fma(S, scale, -ref), weighs the greatest key not by 1 but by 2 to the rounding error of ref: up to 2^4 where scores
+// reach 2^27, and past fp16, or zero, beyond. Waves whose queries could have such scores (on keys of 65504) round S scale to
+// fp32 first, as the few rows' path does.
+constexpr float kFar = 134217728.0f;
+
+__device__ __forceinline__ void scale_first(float16v& s, float scale) {
+  asm volatile("");
+#pragma unroll
+  for (int e = 0; e < 16; ++e) s[e] = mul_rounded(s[e], scale);
+}
+
 __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -286,6 +297,18 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
     };
     wait_stages<PER16, kRing - 2>(min(n - 1, kRing - 2));
     ring_barrier();
+    // The sum of a row's |q| says what scores it could have.
+    float size = 0.0f;
+#pragma unroll
+    for (int i = 0; i < MK; ++i) {
+      const uint4v bits = __builtin_bit_cast(uint4v, qb[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        size = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, bits[e] & 0x7fff7fffu), half2_t{1, 1}, size, false);
+    }
+    const bool far = __ballot(row_sum(size) * 65504.0f * a.scale_log2 >= kFar) != 0;
+    const float by = far ? 1.0f : a.scale_log2;
+    const int plain = far ? 0 : all;  // the scores of steps up to here are left as they come
     const bool busy = (g.tile * kWaves + w) * kStrip < g.members * G;  // a wave without rows only brings tiles
     read_k(0);
     scores();
@@ -302,9 +325,12 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
       if (more) read_k((SLOT + 1) % kRing);
       __builtin_amdgcn_sched_barrier(0);
       const int k0 = g.begin + j * kStep;
-      if (k0 + kStep > all) mask_keys(s, k0, g.begin, lim);
+      if (k0 + kStep > plain) {
+        if (far) scale_first(s, a.scale_log2);
+        if (k0 + kStep > all) mask_keys(s, k0, g.begin, lim);
+      }
       half8 p[2], v[2][DT];
-      weigh(st, s, p, a.scale_log2);
+      weigh(st, s, p, by);
       read_v<D>(v, ring + SLOT * 2 * TILE + TILE);
       __builtin_amdgcn_sched_barrier(0);
       if (more) scores();

@@ -1,0 +1,84 @@
+"""rh_shared_prefix_attention where fp32 scores or fp16 weights come to their ends."""
+import math
+
+import numpy as np
+import pytest
+
+from helpers import bits_to_f32, f16_bits
+from test_shared_prefix import Call, Case
+
+gpu = pytest.mark.gpu
+
+
+def run(torch, dev, case, tol_of, **kw):
+    """The call against attention in 64 bits; tol_of(o, w|v|, keys, max|v|, score size) is a value's tolerance."""
+    print(f"shared prefix: groups={[(g[1], g[2]) for g in case.groups][:6]} n={case.n} {case.heads}/{case.kv_heads} D={case.D} bs={case.bs} {kw}", flush=True)
+    call = Call(torch, dev, case, **kw)
+    call()
+    torch.cuda.synchronize()
+    got = call.out.cpu().numpy().astype(np.float64)
+    q, k, v = (bits_to_f32(x).astype(np.float64) for x in (case.q, case.k, case.v))
+    G, D = case.heads // case.kv_heads, case.D
+    for (row, c, _, _), where in zip(case.meta, case.keys):
+        b, s = (np.array(x) for x in zip(*where))
+        for h in range(case.heads):
+            K, V, x = k[b, h // G, s], v[b, h // G, s], q[row, h * D:(h + 1) * D]
+            logit = K @ x / math.sqrt(D)
+            w = np.exp(logit - logit.max())
+            w /= w.sum()
+            o, a = w @ V, w @ np.abs(V)
+            off = np.abs(got[row, h * D:(h + 1) * D] - o)
+            tol = tol_of(o, a, c, np.abs(V).max(), (np.abs(K) @ np.abs(x)).max() / math.sqrt(D))
+            assert np.isfinite(off).all(), f"row {row}, head {h}: not finite"
+            assert (off <= tol).all(), f"row {row}, head {h}: off by {off.max()}, {np.max(off / tol)} of the tolerance"
+
+
+def equal_weights(o, a, c, v, size):
+    """Of keys whose scores are equal or too far apart to count: the weights' rounding to fp16, the sums' at most 64 roundings of 2^-24 and the
+    result's to fp16, 2^-11 (2^-25 where it is subnormal)."""
+    return 2.0 ** -11 * np.abs(o) + 2.0 ** -25 + (2.0 ** -11 + 64 * 2.0 ** -24) * a
+
+
+@gpu
+@pytest.mark.parametrize("exponent", [9, 11, 12, 15])
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("members,shared,own", [(9, 700, 90), (2, 300, 500)])
+def test_scores_past_fp32s_whole_numbers(torch_mod, dev, members, shared, own, D, exponent):
+    """q is 2^exponent and K +-1.75 of it throughout, so every product and every sum of a score is exact in fp32 and its rounding after the scale
+    is the same for all keys of one score: the keys of the greater score count alike, the others not at all."""
+    case = Case([(members, shared), (1, 0)], [own, max(1, own // 3)], 8, 2, D, seed=members + D)
+    r = np.random.default_rng(exponent)
+    case.q[:] = f16_bits(np.float32(2.0 ** exponent))
+    sign = np.where(r.random(case.k.shape[:3]) < 0.5, 1, -1).astype(np.float32)
+    case.k[:] = f16_bits(np.broadcast_to(sign[..., None] * np.float32(1.75 * 2.0 ** exponent), case.k.shape))
+    run(torch_mod, dev, case, equal_weights)
+
+
+@gpu
+@pytest.mark.parametrize("members", [9, 2])
+@pytest.mark.parametrize("up", [True, False])
+def test_scores_that_grow_or_fall_along_the_keys(torch_mod, dev, members, up):
+    """Key j has K = 1.25 * 2^e with e from -14 to 15, up or down, 20 keys of each: scores from 2^4 to 2^33, doubled from one to the next, so that only
+    the keys of the greatest count."""
+    case = Case([(members, 520)], [80], 8, 2, 64, seed=members)
+    case.q[:] = f16_bits(np.float32(2.0 ** 15))
+    for rows in case.keys:
+        for j, (b, s) in enumerate(rows):
+            case.k[b, :, s] = f16_bits(np.float32(1.25 * 2.0 ** (j // 20 - 14 if up else 15 - j // 20)))
+    run(torch_mod, dev, case, equal_weights)
+
+
+@gpu
+@pytest.mark.parametrize("members", [9, 2])
+def test_scores_far_apart_in_one_wave(torch_mod, dev, members):
+    """Heads of scores past 2^24, of either sign, beside heads of scores of up to 36. K is +-1.5 * 2^10 for kv head 0, 1.75 * 2^14 for kv head 1: exact sums
+    and two scores, or one, for every row. Small scores have a score's usual error besides, and their smaller weights 2^-25."""
+    case = Case([(members, 640)], [70], 8, 2, 64, seed=members)
+    q, k, r = bits_to_f32(case.q).reshape(-1, 8, 64), bits_to_f32(case.k), np.random.default_rng(3)
+    q[:, :3] = np.array([1, 2, 3])[:, None] * 2.0 ** -10
+    q[:, 3] = 2.0 ** 15
+    q[:, 5] = -2.0 ** 15
+    k[:, 0] = np.where(r.random(k[:, 0].shape[:2]) < 0.3, 1, -1)[..., None] * 1.5 * 2.0 ** 10
+    k[:, 1] = 1.75 * 2.0 ** 14
+    case.q, case.k = f16_bits(q).reshape(case.q.shape), f16_bits(k)
+    run(torch_mod, dev, case, lambda o, a, c, v, size: equal_weights(o, a, c, v, size) + (c * 2.0 ** -25 * v + 2 * 66 * 2.0 ** -24 * size * a if size < 100 else 0))
