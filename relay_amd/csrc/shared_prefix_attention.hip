@@ -85,19 +85,23 @@ __device__ __forceinline__ int kswz(int key) {
 template <int D>
 struct Strip {
   float16v o[D / 32];
-  float ref, l;  // the row's maximum in the log2 domain (-inf: no key seen), this lane's share of its sum
+  float ref, l;  // the offset of the row's weights in the log2 domain (-inf: no key seen), this lane's share of their sum
 };
 
-// P = exp2(S scale - ref) with the row's running maximum as ref, and the sum. O and l are rescaled where a
+// Weights are 2^kUp for the greatest score so far: as fp16 they then keep their 11 bits down to 2^-25 of it and end at 2^-36. (With 1
+// for the greatest they end at 2^-25: one key that outweighs each of many others by that much, and the others were lost.)
+constexpr float kUp = 11.0f;
+
+// P = exp2(S scale - ref) with the row's running maximum less `up` as ref, and the sum. O and l are rescaled where a
 // row of the wave has a new maximum: on fewer and fewer steps. (An offset that moved only before a
 // weight could overflow fp16 took up to 5% less time, and doubled the noise of the weights' rounding:
-// with a maximum as offset the greatest weight, which counts most, is exactly 1.) A masked key's S is -inf.
+// with a maximum as offset the greatest weight, which counts most, is a power of two.) A masked key's S is -inf.
 template <int D>
-__device__ __forceinline__ void weigh(Strip<D>& st, const float16v& s, half8 (&p)[2], float scale) {
+__device__ __forceinline__ void weigh(Strip<D>& st, const float16v& s, half8 (&p)[2], float scale, float up) {
   float mx = s[0];
 #pragma unroll
   for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
-  mx = row_max(mx) * scale;
+  mx = row_max(mx) * scale - up;
   if (__ballot(mx > st.ref) != 0) {
     const float ref = fmaxf(mx, st.ref), alpha = ref == -INFINITY ? 1.0f : fast_exp2(st.ref - ref);
     st.ref = ref;
@@ -156,9 +160,9 @@ __device__ __forceinline__ void mask_keys(float16v& s, int key0, int lo, int lim
   }
 }
 
-// One fma a score, fma(S, scale, -ref), weighs the greatest key not by 1 but by 2 to the rounding error of ref: up to 2^4 where scores
-// reach 2^27, and past fp16, or zero, beyond. Waves whose queries could have such scores (on keys of 65504) round S scale to
-// fp32 first, as the few rows' path does.
+// One fma a score, fma(S, scale, -ref), is off for the greatest key by the rounding error of ref: up to 4 where scores reach 2^27,
+// and beyond by more than fp16's range. Waves whose queries could have such scores (on keys of 65504) round S scale to fp32
+// first, as the few rows' path does, and weigh the greatest by 1.
 constexpr float kFar = 134217728.0f;
 
 __device__ __forceinline__ void scale_first(float16v& s, float scale) {
@@ -307,7 +311,7 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
         size = __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, bits[e] & 0x7fff7fffu), half2_t{1, 1}, size, false);
     }
     const bool far = __ballot(row_sum(size) * 65504.0f * a.scale_log2 >= kFar) != 0;
-    const float by = far ? 1.0f : a.scale_log2;
+    const float by = far ? 1.0f : a.scale_log2, up = far ? 0.0f : kUp;
     const int plain = far ? 0 : all;  // the scores of steps up to here are left as they come
     const bool busy = (g.tile * kWaves + w) * kStrip < g.members * G;  // a wave without rows only brings tiles
     read_k(0);
@@ -330,7 +334,7 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
         if (k0 + kStep > all) mask_keys(s, k0, g.begin, lim);
       }
       half8 p[2], v[2][DT];
-      weigh(st, s, p, by);
+      weigh(st, s, p, by, up);
       read_v<D>(v, ring + SLOT * 2 * TILE + TILE);
       __builtin_amdgcn_sched_barrier(0);
       if (more) scores();
@@ -513,7 +517,8 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
           mx = fmaxf(mx, x[4 * t + e]);
         }
       }
-      mx = fmaxf(ref, group4_max(mx));
+      mx = group4_max(mx);
+      mx = fmaxf(ref, fabsf(mx) < 1048576.0f ? mx - kUp : mx);  // (2^20: past it kUp comes to be lost in rounding)
       const float base = mx == -INFINITY ? 0.0f : mx, alpha = fast_exp2(ref - base);
       ref = mx;
       half8 p;

@@ -82,3 +82,21 @@ def test_scores_far_apart_in_one_wave(torch_mod, dev, members):
     k[:, 1] = 1.75 * 2.0 ** 14
     case.q, case.k = f16_bits(q).reshape(case.q.shape), f16_bits(k)
     run(torch_mod, dev, case, lambda o, a, c, v, size: equal_weights(o, a, c, v, size) + (c * 2.0 ** -25 * v + 2 * 66 * 2.0 ** -24 * size * a if size < 100 else 0))
+
+
+@gpu
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("members,shared,own,hints", [(9, 20000, 40, (9, 128, 40)), (2, 1000, 12000, (2, 128, 0)), (1, 0, 9000, (1, 0, 0)), (40, 6000, 20, None)])
+def test_many_keys_far_below_one(torch_mod, dev, members, shared, own, hints, D):
+    """Key 0 has a score of 18, value 0; all others 0, with values of one sign: e^-18 = 2^-26 of key 0's weight each, and all of the result.
+    Each weight is rounded to fp16, 2^-11 of it, or 2^-25 of 2^-11 of the greatest where that is subnormal; scores are exact but for their
+    scale (2 (D + 2) 2^-24 of their size); sums and result as elsewhere."""
+    case = Case([(members, shared)], [own], 8, 2, D, seed=D + members)
+    q, k, v = np.zeros((members, 8, D)), np.zeros(case.k.shape), np.abs(bits_to_f32(case.v)) + 0.25
+    q[:, :, 0] = 2.0 * math.sqrt(D) if D != 128 else 22.625  # a score of 17.998 there
+    for b, s in {rows[0] for rows in case.keys}:
+        k[b, :, s, 0] = 9.0
+        v[b, :, s] = 0.0
+    case.q, case.k, case.v = f16_bits(q).reshape(case.q.shape), f16_bits(k), f16_bits(v)
+    run(torch_mod, dev, case, lambda o, a, c, v, size: 2.0 ** -11 * np.abs(o) + 2.0 ** -25 + c * 2.0 ** -36 * v
+        + (2.0 ** -11 + 2 * (D + 2) * 2.0 ** -24 * size + 64 * 2.0 ** -24) * a, hints=hints)
