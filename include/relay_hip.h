@@ -475,7 +475,10 @@ int rh_kv_scatter_from_host(void* kpool, void* vpool, const int* blocks, int n, 
 /* Block tables and slot maps of a step, from the lengths of its sequences.
  *  cached [n_seqs]      tokens of each sequence that the cache holds
  *  fresh  [n_seqs]      tokens that this step adds (0: the sequence waits)
- *  shared [n_seqs]      leading keys that its group shares, which are in the cache (NULL: none)
+ *  shared [n_seqs]      leading keys that its group shares (NULL: none), of a group's first sequence at most
+ *                       the keys that its cache holds when attention reads them: they are read through
+ *                       its row of `tables`. More than a row holds is refused; more than the sequence
+ *                       holds is not, and attention then reads the entries behind its blocks
  *  group_seqs [n_groups][2]  first sequence and number of sequences of each group
  *  tables [n_seqs][table_stride]  block ids; sequence s holds ceil(cached[s] / block_size) on
  *                       entry and ceil((cached[s] + fresh[s]) / block_size) afterwards
@@ -500,7 +503,8 @@ enum {
   RH_STEP_ROWS_FULL = 1,  /* more than max_rows tokens */
   RH_STEP_NO_BLOCKS = 2,  /* more blocks than the stack holds */
   RH_STEP_TABLE_FULL = 4, /* a sequence past table_stride blocks */
-  RH_STEP_BAD_LENGTH = 8  /* a negative or too large length, a group that is no range of sequences */
+  RH_STEP_BAD_LENGTH = 8  /* a negative or too large length, a group that is no range of sequences; and, if nothing
+                           * else is wrong, more shared keys than a row of the tables holds */
 };
 int rh_step_tables(const int* cached, const int* fresh, const int* shared, int n_seqs, const int* group_seqs, int n_groups,
                    int block_size, int* tables, int table_stride, const int* free_blocks, const int* free_count,
@@ -530,7 +534,9 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
  *                        of the table that the shared keys are read through
  * A token attends to keys 0 .. context - 1: those below its shared keys through its group's table,
  * the others through its own. It belongs to exactly one group if its shared keys are positive, and
- * they are the group's. A group's table holds all its shared keys, written and finite; a member's
+ * they are the group's. A group's table holds all its shared keys, written and finite (an entry that
+ * holds no block, if it has one, must be negative or a block of the pools: a negative one is read as
+ * block 0, so that the call stays inside the pools, but its result means nothing); a member's
  * context may end before them. A token of context 0 is idle, its row left as it was. Several
  * tokens of one sequence are several entries, each with a row of its own.
  *  max_members, max_shared, max_own  the largest group, the most shared keys and the most keys

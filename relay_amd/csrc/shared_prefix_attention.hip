@@ -197,6 +197,10 @@ struct Share {
 
 typedef const __attribute__((address_space(4))) int* scalar_ints;  // uniform reads go through the scalar unit
 
+// The block of a table's entry. Entries that hold none may be any negative number: they lead to block 0 and not outside the pools
+// where a group is said to share more keys than its table has (a max a table entry costs nothing measurable).
+__device__ __forceinline__ int block_at(int entry) { return max(entry, 0); }
+
 // ---- many rows: the waves share tiles of K and V in LDS, 32 rows a wave ---------------------------
 //
 //   S^T[32 keys x 32 rows] = K[32 keys x D] * Q^T[D x 32 rows]          (MFMA 32x32x16)
@@ -228,7 +232,7 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
     // A wave brings half a tile's K or V, 16 keys of one table entry, which it looks up a tile ahead.
     int entry;
     const auto first16 = [&](int j) { return min(g.begin + j * kStep + 16 * (w & 1), (g.end - 1) & ~15); };
-    const auto lookup = [&](int j) { entry = entries[first16(j) >> sh]; };
+    const auto lookup = [&](int j) { entry = block_at(entries[first16(j) >> sh]); };
     uint32_t piece[PER16];  // a lane's offsets in 16 keys
     const auto pieces_to = [&](int last) {
 #pragma unroll
@@ -423,7 +427,7 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
     const auto head_of = [&](int row) { return sh.kvh * G + (pieces == 1 ? row - a.by_group(row) * G : head0 + row); };
     const auto row_any = [&](int j) -> unsigned {
       j = min(j, end - 1);
-      return (static_cast<unsigned>(sh.table[bshift >= 0 ? j >> bshift : j / bs]) * a.kv_heads + sh.kvh) * bs +
+      return (static_cast<unsigned>(block_at(sh.table[bshift >= 0 ? j >> bshift : j / bs])) * a.kv_heads + sh.kvh) * bs +
              (bshift >= 0 ? j & (bs - 1) : j % bs);
     };
     // SCALAR: the table entries of the two 16-key runs of a step, looked up a step ahead. The first
@@ -431,7 +435,7 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
     int entry[2];
     const auto run_of = [&](int k0, int t) { return min(k0 + 16 * t, (end - 1) & ~15); };
     const auto lookup = [&](int k0) {
-      if (SCALAR) entry[0] = entries[run_of(k0, 0) >> bshift], entry[1] = entries[run_of(k0, 1) >> bshift];
+      if (SCALAR) entry[0] = block_at(entries[run_of(k0, 0) >> bshift]), entry[1] = block_at(entries[run_of(k0, 1) >> bshift]);
     };
     const auto issue = [&](KvStep<D, DR>& st, int k0) {
       const auto row_of = [&](int t, int off) -> unsigned {

@@ -37,7 +37,7 @@ struct StepArgs {
   int n_seqs, n_groups, block;
   Div by_block;
   int* tables;
-  int stride;
+  int stride, row_keys;  // entries of a sequence's row of the tables, and keys that they hold
   const int *free_blocks, *free_count;
   int max_rows;
   int *row_off, *last_row, *table_off, *pos, *seq, *slot;
@@ -80,15 +80,21 @@ struct Length {
   Need need;
 };
 
+constexpr int kPastTable = 16;  // more shared keys than a row of the tables holds: attention would read past it
+
+// The call's status: what is wrong with its lengths and its room, else with its shared keys.
+__device__ __forceinline__ int status_of(int bad) { return bad & (kPastTable - 1) ? bad & (kPastTable - 1) : bad ? RH_STEP_BAD_LENGTH : 0; }
+
 // What sequence s adds, or why it cannot.
 __device__ __forceinline__ Length length_of(const StepArgs& a, int s) {
   Length n{a.cached[s], a.shared ? a.shared[s] : 0, 0, {0, 0}};
   const int f = a.fresh[s];
+  if (n.shared > a.row_keys) n.bad = kPastTable;
   if (n.cached < 0 || f < 0 || n.cached > kSumCap || f > kSumCap - n.cached || n.shared < 0) {
-    n.bad = RH_STEP_BAD_LENGTH;
+    n.bad |= RH_STEP_BAD_LENGTH;
   } else {
     const int want = blocks_of(n.cached + f, a.by_block);
-    if (want > a.stride) n.bad = RH_STEP_TABLE_FULL;
+    if (want > a.stride) n.bad |= RH_STEP_TABLE_FULL;
     n.need = {f, want - blocks_of(n.cached, a.by_block)};
   }
   return n;
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(THREADS) void step_tables_kernel(const StepArgs a) 
   if (bad) atomicOr(&s_bad, bad);
   if (most > kOwnRows) s_most = 1;
   __syncthreads();
-  const int status = s_bad;
+  const int status = status_of(s_bad);
   const bool own_rows = ROWS && !s_most;
   if (status) all = {0, 0};
 
@@ -284,7 +290,7 @@ __global__ __launch_bounds__(THREADS) void step_wide_kernel(const StepArgs a) {
   if (a.n_seqs == 0) __syncthreads();  // (the scans' barriers follow s_bad's clearing)
   if (bad) atomicOr(&s_bad, bad);
   __syncthreads();
-  const int status = s_bad;
+  const int status = status_of(s_bad);
   if (status) all = {0, 0};
   const auto last_at = [&](const int* firsts, int k) {  // the last sequence that begins at or before k
     int lo = 0, hi = a.n_seqs;
@@ -750,8 +756,8 @@ int rh_step_tables(const int* cached, const int* fresh, const int* shared, int n
              "step tables: missing pointer");
   RH_REQUIRE((reinterpret_cast<uintptr_t>(dec_meta) | reinterpret_cast<uintptr_t>(groups)) % 16 == 0,
              "step tables: dec_meta and groups must be 16-byte aligned");
-  const StepArgs a{cached, fresh, shared, group_seqs, n_seqs, n_groups, block_size, div_by(block_size), tables, table_stride, free_blocks,
-                   free_count, max_rows, row_off, last_row, table_off, pos, seq, slot,
+  const StepArgs a{cached, fresh, shared, group_seqs, n_seqs, n_groups, block_size, div_by(block_size), tables, table_stride,
+                   static_cast<int>(std::min<int64_t>(static_cast<int64_t>(table_stride) * block_size, INT32_MAX)), free_blocks, free_count, max_rows, row_off, last_row, table_off, pos, seq, slot,
                    reinterpret_cast<int4*>(dec_meta), reinterpret_cast<int4*>(groups), totals};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, dim3(1), dim3(threads), 0, s, a); };
