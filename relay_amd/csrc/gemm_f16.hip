@@ -146,10 +146,9 @@ __global__ __launch_bounds__(WN * WT * WK * 64, 1) void gemm_f16_kernel(const ha
       mma(q & 1);
     }
     if (s + 1 < nsteps) {
-      // Every read of stage s has landed in registers, stage s + 1 has landed in LDS (in
-      // flight behind it: stages s + 2 .. s + AHEAD - 1 ...); after the barrier both hold
-      // for all waves, and stage s's buffer takes stage s + STAGES.
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
+      // Stage s + 1 has landed in LDS (in flight behind it: stages s + 2 .. s + AHEAD - 1 ...) and,
+      // with the barrier's own wait, every read of stage s in registers; after the barrier both
+      // hold for all waves, and stage s's buffer takes stage s + STAGES.
       wait_stages<LPS, STAGES - 2>(nsteps - 2 - s);
       ring_barrier();
       read(nbuf, 0, 0);
@@ -160,7 +159,6 @@ __global__ __launch_bounds__(WN * WT * WK * 64, 1) void gemm_f16_kernel(const ha
   if constexpr (WK == 2) {
     // Waves w and w + WN WT hold the two K halves of the same blocks: each keeps every other
     // block and hands the rest over through LDS.
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     ring_barrier();
     float* const xs = reinterpret_cast<float*>(lds) + (w % (WN * WT)) * (AN * AT * 1024) + lane * 4;
 #pragma unroll
@@ -171,7 +169,6 @@ __global__ __launch_bounds__(WN * WT * WK * 64, 1) void gemm_f16_kernel(const ha
           *reinterpret_cast<float4v*>(xs + i * 1024 + q * 256) =
               float4v{acc[i / AT][i % AT][4 * q], acc[i / AT][i % AT][4 * q + 1], acc[i / AT][i % AT][4 * q + 2],
                       acc[i / AT][i % AT][4 * q + 3]};
-    asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     ring_barrier();
 #pragma unroll
     for (int i = 0; i < AN * AT; ++i)

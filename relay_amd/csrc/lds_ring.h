@@ -1,5 +1,5 @@
 // Global memory -> LDS loads without registers, and the waits of a ring of LDS buffers fed by
-// them (the tile product of gemm_f16.hip).
+// them (the tile products of gemm_f16.hip, the shared prefixes of shared_prefix_attention.hip).
 #pragma once
 
 #include "common.h"
@@ -43,10 +43,11 @@ __device__ __forceinline__ void wait_stages(int later) {
   }
 }
 
-// A workgroup barrier after which LDS contents written by any wave's landed loads are visible,
-// and no LDS access moves across it.
+// A workgroup barrier after which LDS contents written by any wave's landed loads are visible, no LDS access
+// moves across it, and every wave's LDS reads before it have landed: their buffer may be loaded into again. (gfx950
+// does not wait for them at a barrier, and the compiler waits where their values are used, which may be behind it.)
 __device__ __forceinline__ void ring_barrier() {
-  asm volatile("" : : : "memory");
+  asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" : : : "memory");
 }
