@@ -554,8 +554,10 @@ int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, const void* 
 size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_members, int max_shared, int max_own, int heads,
                                   int kv_heads, int head_dim);
 
-/* 1 where sharing is measured to be faster than rh_paged_decode_attention on the same dec_meta (whose
- * fourth values that ignores) and tables, if every token's own table holds its whole context. */
+/* 1 where sharing should be faster than rh_paged_decode_attention on the same dec_meta (whose fourth
+ * values that ignores) and tables, if every token's own table holds its whole context: a rule from
+ * timings of 2000 shapes, right in 97 of 100 that it answers with 1 (groups of two are most of the rest).
+ * 0 for one token, which shares nothing. */
 int rh_shared_prefix_pays(int n_dec, int max_shared, int max_own, int heads, int kv_heads, int head_dim);
 
 /* Host-side: which tokens of a step share a prefix. tokens [n_dec][4] are rh_paged_decode_attention's

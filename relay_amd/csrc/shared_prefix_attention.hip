@@ -870,16 +870,23 @@ size_t bytes_of(const Plan& p, int n_dec, int heads, int head_dim) {
 using namespace relay_hip;
 
 extern "C" int rh_shared_prefix_pays(int n_dec, int max_shared, int max_own, int heads, int kv_heads, int head_dim) {
-  if (n_dec <= 0 || max_shared <= 0 || max_own < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
-  // What each token reads by itself, of which all but one reading of a prefix come from the caches: up to 100
-  // MB the decode kernel's one launch and smaller steps win. Measured (us, decode / shared; members x shared +
-  // own): 32/8 heads of 128, 4 x 4096 + 304 (70 MB) 15.2 / 19.0, 16 x 1024 + 200 (76) 14.3 / 15.5, 24 x 1024 + 100
-  // (107) 21 / 16, 32 x 1024 + 300 (160) 28 / 20, 32 x 4096 + 300 (562) 58 / 25; 32/4 of 64, 32 x 1024 + 300 (40) 10.3 / 13.1, 8
-  // groups of 4 x 3008 + 300 (105) 17.6 / 16.9, 32 x 4096 + 300 (141) 18.4 / 17.6, 64 x 2048 + 500 (156) 21 / 18; 9/3 of 64, 64 x
-  // 512 + 100 (28) 11.6 / 11.5, 32 x 4096 + 300 (105) 21 / 15.
-  // 16 query heads of 128 a kv head merge slowly there: 16/1, 2 x 4096 + 100 23 / 16, 64 x 512 + 100 13.6 / 15.3.
-  const double alone = static_cast<double>(n_dec) * kv_heads * head_dim * 4 * (max_shared + 0.65 * max_own);
-  return alone > 100e6 || static_cast<int64_t>(heads / kv_heads) * head_dim > 1024;
+  // One token shares nothing.
+  if (n_dec < 2 || max_shared <= 0 || max_own < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
+  // The decode kernel reads each token's keys, once for each 16 query heads of a kv head (at head size 32 the caches hide
+  // that); here a prefix is read once, but own keys take some 10% longer and most calls a second launch. So sharing pays where
+  // the readings saved, less what own keys lose, pass a number of bytes, fewer where there are many workgroups. Measured (us,
+  // decode / shared; members x shared + own; MB saved): 32/8 heads of 128, 4 x 4096 + 304 (50) 15.2 / 19.0, 16 x 1024 + 200 (63) 14.3 /
+  // 15.5, 24 x 1024 + 100 (96) 21 / 16, 32 x 1024 + 300 (130) 28 / 20, 48 x 1024 + 4000 98 / 108 and 105 / 108 with 256 shared; 32/4 of 64, 32 x
+  // 1024 + 300 (32) 10.3 / 13.1, 48 x 1024 + 1000 (49) 19 / 17, 48 x 4096 + 16,000 113 / 114; 9/3 of 64, 104 tokens on 672 + 13 (53) 18.3 / 11.2.
+  // Of 1500 shapes with groups of three and more members the rule makes 33 slower, by 5% on average and 25% at worst, and leaves
+  // 180 that sharing would make faster by 12% on average; of 460 with groups of two, which save half, 19 slower, 24% at worst.
+  const int group = heads / kv_heads;
+  const double pieces = head_dim >= 64 ? (group + 15) / 16 : 1, units = pieces * n_dec * kv_heads;
+  const double saved = 4.0 * head_dim * kv_heads * pieces * ((n_dec - 1.0) * max_shared - 0.26 * (n_dec + 4.0) * max_own);
+  if (saved > (units >= 192 ? 45e6 : 70e6)) return 1;
+  // Few workgroups of wide kv heads merge their slices slowly there: 16/1 of 128, 2 x 2048 + 40 18.3 / 13.7, 2 x 4096 + 100 23 / 16,
+  // 16 x 4096 + 100 23.5 / 18.3, but 16 x 1024 + 300 13.1 / 14.2, 64 x 512 + 100 13.6 / 15.3; 32/2, 16 x 2048 + 40 16.0 / 17.3.
+  return head_dim == 128 && group * head_dim > 1024 && max_shared >= 2000 && units <= 24;
 }
 
 extern "C" int rh_shared_prefix_groups(const int* tokens, const int* tables, int n_dec, int block_size, int min_shared,

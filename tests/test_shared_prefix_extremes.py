@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 from helpers import bits_to_f32, f16_bits
+from relay_amd import _lib
 from test_shared_prefix import Call, Case
 
 gpu = pytest.mark.gpu
@@ -100,3 +101,31 @@ def test_many_keys_far_below_one(torch_mod, dev, members, shared, own, hints, D)
     case.q, case.k, case.v = f16_bits(q).reshape(case.q.shape), f16_bits(k), f16_bits(v)
     run(torch_mod, dev, case, lambda o, a, c, v, size: 2.0 ** -11 * np.abs(o) + 2.0 ** -25 + c * 2.0 ** -36 * v
         + (2.0 ** -11 + 2 * (D + 2) * 2.0 ** -24 * size + 64 * 2.0 ** -24) * a, hints=hints)
+
+
+# (tokens, shared, own, heads, kv heads, head size), and us of rh_paged_decode_attention / this as measured
+MEASURED = [
+    ((16, 1024, 300, 16, 1, 128), 13.1, 14.2), ((64, 512, 100, 16, 1, 128), 13.6, 15.3), ((16, 2048, 40, 32, 2, 128), 16.0, 17.3),
+    ((64, 512, 100, 32, 2, 128), 14.3, 17.1), ((64, 16, 60, 64, 4, 128), 6.9, 15.9), ((64, 512, 100, 12, 1, 128), 12.4, 14.7),
+    ((48, 16, 4000, 32, 8, 128), 97.9, 107.8), ((48, 16, 4000, 32, 4, 64), 28.3, 32.6), ((2, 4096, 16000, 8, 8, 128), 23.6, 30.2),
+    ((30, 2672, 267, 32, 1, 128), 24.9, 20.0), ((100, 7104, 142, 12, 1, 128), 52.8, 28.6), ((3, 3392, 3392, 64, 4, 128), 39.8, 19.6),
+    ((87, 4864, 4864, 32, 1, 128), 125.1, 70.9), ((18, 16032, 320, 64, 4, 128), 72.3, 42.5), ((79, 17728, 1772, 32, 1, 128), 163.2, 61.8),
+    ((5, 10176, 203, 64, 2, 128), 42.7, 23.2), ((104, 784, 1176, 28, 4, 128), 72.7, 42.1), ((14, 3776, 75, 8, 8, 64), 16.6, 12.7),
+    ((51, 304, 152, 8, 8, 128), 19.1, 15.5), ((75, 5888, 5888, 16, 8, 32), 86.2, 67.5), ((120, 1008, 100, 28, 4, 128), 52.6, 22.7),
+    ((48, 4096, 4000, 28, 4, 128), 102.0, 70.9), ((55, 352, 176, 8, 8, 128), 21.1, 16.3), ((4, 512, 100, 64, 2, 64), 9.6, 11.3),
+    ((16, 512, 100, 40, 1, 32), 5.8, 10.0), ((16, 1024, 300, 40, 1, 32), 8.8, 10.3), ((16, 1024, 300, 12, 1, 128), 11.9, 14.1),
+    ((16, 512, 100, 64, 2, 64), 8.0, 11.7), ((64, 16, 60, 40, 1, 64), 5.7, 10.7), ((16, 16, 60, 40, 1, 64), 5.5, 9.5),
+    ((3, 13232, 19848, 8, 8, 64), 25.9, 30.1), ((27, 336, 33, 64, 8, 128), 13.6, 16.3), ((32, 1728, 864, 16, 4, 32), 10.4, 12.6),
+    ((48, 4096, 16000, 9, 3, 64), 89.5, 104.6), ((8, 4176, 2088, 32, 4, 64), 12.2, 16.6), ((48, 16, 4000, 32, 4, 64), 28.1, 32.6),
+    ((48, 16, 4000, 14, 2, 64), 19.3, 22.4)]
+
+
+@pytest.mark.parametrize("shape,decode,shared", MEASURED)
+def test_sharing_pays_says_what_was_measured(shape, decode, shared):
+    assert _lib.lib().rh_shared_prefix_pays(*shape) == (shared < decode)
+
+
+@pytest.mark.parametrize("shared", [1, 16, 16384, 1 << 30])
+def test_one_token_shares_nothing(shared):
+    for heads, kv_heads, D in ((16, 1, 128), (32, 8, 128), (40, 1, 64)):
+        assert _lib.lib().rh_shared_prefix_pays(1, shared, 0, heads, kv_heads, D) == 0
