@@ -106,23 +106,21 @@ def exact(case, seed):
 
 
 def _own_call(state, name, build):
-    """The bound call of a state: a program that decodes step after step keeps its argument list and workspaces."""
+    """The bound call of a state, on the current stream: a program that decodes step after step keeps its argument list, workspaces and
+    output buffers (so the next run writes what this one returned) and looks up no more than its stream."""
     if "call" not in state:
         from relay_amd import _lib
         fn, args, check = getattr(_lib.lib(), name), build(_lib.lib()), _lib.check
+        stream, device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device()
 
         def call():
-            check(fn(*args), name)
+            check(fn(*args, stream(device)), name)
         state["call"] = call
     state["call"]()
 
 
 def _p(t):
     return 0 if t is None else t.data_ptr()
-
-
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
 
 
 # ---- attention over a shared prefix ---------------------------------------------------------------
@@ -187,8 +185,7 @@ def _own_shared(s):
         size = lib.rh_shared_prefix_workspace(n, ng, c["members"], c["shared"], s["max_own"], heads, kvh, d)
         s["workspace"] = torch.zeros(max(1, size), dtype=torch.uint8, device=DEV)
         return (_p(s["q"]), heads * d, _p(s["k"]), _p(s["v"]), _p(s["meta"]), _p(s["groups"]), _p(s["tables"]), n, ng, c["members"],
-                c["shared"], s["max_own"], heads, kvh, d, c["block"], 1.0 / math.sqrt(d), _p(s["workspace"]), size, _p(s["out"]), heads * d,
-                _stream())
+                c["shared"], s["max_own"], heads, kvh, d, c["block"], 1.0 / math.sqrt(d), _p(s["workspace"]), size, _p(s["out"]), heads * d)
     _own_call(s, "rh_shared_prefix_attention", build)
     return s["out"]
 
@@ -300,7 +297,7 @@ def _own_tables(s):
         c = s["case"]
         return (_p(s["cached"]), _p(s["fresh"]), _p(s["shared"]), c["seqs"], _p(s["group_seqs"]) if c["groups"] else 0, c["groups"], c["block"],
                 _p(s["tables"]), s["tables"].shape[1], _p(s["free"]), _p(s["free_count"]), s["rows"], _p(s["row_off"]), _p(s["last_row"]),
-                _p(s["table_off"]), _p(s["pos"]), _p(s["seq"]), _p(s["slot"]), _p(s["meta"]), _p(s["groups"]), _p(s["totals"]), _stream())
+                _p(s["table_off"]), _p(s["pos"]), _p(s["seq"]), _p(s["slot"]), _p(s["meta"]), _p(s["groups"]), _p(s["totals"]))
     _own_call(s, "rh_step_tables", build)
     return _tables_outputs(s)
 
@@ -358,7 +355,7 @@ def _own_qk_norm(s):
     def build(lib):
         c = s["case"]
         return (_p(s["qkv"]), c["planes"], 0, c["tokens"], _p(s["bias"]), _p(s["q_norm"]), _p(s["k_norm"]), EPS, _p(s["inv_freq"]), _p(s["pos"]),
-                _p(s["slot"]), _p(s["k"]), _p(s["v"]), _p(s["q"]), s["q_scale"], c["heads"], c["kv_heads"], c["dim"], s["block"], _stream())
+                _p(s["slot"]), _p(s["k"]), _p(s["v"]), _p(s["q"]), s["q_scale"], c["heads"], c["kv_heads"], c["dim"], s["block"])
     _own_call(s, "rh_qk_norm_to_cache", build)
     return {"q": s["q"], "k": s["k"], "v": s["v"]}
 
@@ -446,7 +443,7 @@ def _own_logits(s):
         return (_p(s["logits"]), v, r, v, _p(s["history"]), c["history"], _p(s["history_len"]), _p(s["prompt_len"]), _p(s["repetition"]),
                 _p(s["frequency"]), _p(s["presence"]), _p(s["bias_tokens"]) if bias else 0, _p(s["bias_values"]) if bias else 0, c["biases"],
                 _p(s["bias_len"]) if bias else 0, _p(s["masks"]) if mask else 0, s["masks"].shape[1], _p(s["mask_of"]) if mask else 0,
-                _p(s["out"]), v, _p(s["next"]), _p(s["workspace"]), size, _stream())
+                _p(s["out"]), v, _p(s["next"]), _p(s["workspace"]), size)
     _own_call(s, "rh_process_logits", build)
     return {"out": s["out"], "next": s["next"]}
 
