@@ -1043,13 +1043,12 @@ extern "C" int rh_shared_prefix_attention(const void* q, int64_t q_row_stride, c
     case 64: if (int rc = launch<64, 64>(a, p.rows, wgs, s)) return rc; break;
     default: if (int rc = launch<128, 128>(a, p.rows, wgs, s)) return rc;
   }
-  if (!p.rows) return 0;
+  if (!p.rows) return 0;  // (as always at head size 16)
   const int64_t values = static_cast<int64_t>(n_dec) * heads * head_dim;
   const auto join = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((values + 255) / 256)), dim3(256), 0, s, a);
   };
   switch (head_dim) {
-    case 16: RH_TRY_LAUNCH(join(shared_join_kernel<16>)); break;
     case 32: RH_TRY_LAUNCH(join(shared_join_kernel<32>)); break;
     case 64: RH_TRY_LAUNCH(join(shared_join_kernel<64>)); break;
     default: RH_TRY_LAUNCH(join(shared_join_kernel<128>));
