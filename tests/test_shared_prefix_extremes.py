@@ -129,3 +129,19 @@ def test_sharing_pays_says_what_was_measured(shape, decode, shared):
 def test_one_token_shares_nothing(shared):
     for heads, kv_heads, D in ((16, 1, 128), (32, 8, 128), (40, 1, 64)):
         assert _lib.lib().rh_shared_prefix_pays(1, shared, 0, heads, kv_heads, D) == 0
+
+
+@gpu
+@pytest.mark.parametrize("D", [16, 64, 128])
+def test_no_groups_at_all(torch_mod, dev, D):
+    """Tokens on their own, with no group array: what rh_shared_prefix_groups leaves where nothing is shared."""
+    case = Case([(1, 0)] * 7, [300, 1, 65, 1100], 8, 2, D, seed=D)
+    want, tol = case.oracle()
+    case.groups = []
+    call = Call(torch_mod, dev, case)
+    args = list(call.args)
+    assert args[8] == 0
+    args[5] = None
+    _lib.check(call.lib.rh_shared_prefix_attention(*args, None))
+    torch_mod.cuda.synchronize()
+    assert (np.abs(call.out.double().cpu().numpy() - want) <= tol).all()

@@ -1,9 +1,10 @@
-"""Steps whose groups share more keys than there are."""
+"""Steps whose groups share more keys than there are, and the forms of the q/k norm and logits kernels that large calls take."""
 import numpy as np
 import pytest
 
 from test_shared_prefix import Call, Case
-from test_step_ops import BAD_LENGTH, NO_BLOCKS, run_tables, same, tables_case, tables_oracle
+from test_step_ops import (BAD_LENGTH, NO_BLOCKS, LogitCase, QkCase, check_logits, check_qk, run_tables, same, tables_case,
+                           tables_oracle)
 
 gpu = pytest.mark.gpu
 
@@ -47,3 +48,26 @@ def test_entries_without_a_block_lead_into_the_pools(torch_mod, dev, members, sh
         if value == 0:
             want = out
         assert torch.equal(out, want) and bool(torch.isfinite(out).all())
+
+
+@gpu
+@pytest.mark.parametrize("T,heads,kv_heads,D", [(2101, 9, 3, 64), (1900, 32, 4, 64), (2503, 20, 5, 32), (1777, 32, 8, 128), (1003, 7, 3, 128), (701, 4, 2, 256),
+                                               (402, 3, 2, 512), (4999, 5, 2, 16)])
+@pytest.mark.parametrize("bias,scale", [(False, False), (True, False), (False, True)])
+def test_qk_norm_two_sets_of_heads_a_wave(torch_mod, dev, T, heads, kv_heads, D, bias, scale):
+    """One plane of many rows, with a last set of heads that is not whole, and idle rows."""
+    assert T * (heads + 2 * kv_heads) * max(4, D // 8) >= 150000
+    check_qk(torch_mod, dev, QkCase(T, heads, kv_heads, D, seed=T, bias=bias, scale=scale, idle=(0, 5, T // 2, T - 1)))
+
+
+@gpu
+@pytest.mark.parametrize("out_ld", [9001, 9003, 9004])
+@pytest.mark.parametrize("biases", [0, 7])
+@pytest.mark.parametrize("rows,history", [(20, 0), (20, 60), (20, 4500), (65, 0), (65, 60), (110, 4500)])
+def test_logits_forms(torch_mod, dev, rows, history, biases, out_ld):
+    """One and two loads a thread, 256 and 512 threads (histories over 4096), with and without biases, rows that lie alike to 16 bytes or not."""
+    case = LogitCase(rows, 9001, history, biases, masks=3, seed=rows + history, ld=9004 if out_ld == 9004 else None)
+    check_logits(torch_mod, dev, case, out_ld=out_ld)
+    check_logits(torch_mod, dev, case, out_ld=out_ld, shift=1)
+    case.mask_of[:] = -1  # (masks that no row uses)
+    check_logits(torch_mod, dev, case, out_ld=out_ld, shift=3, next_=False)
