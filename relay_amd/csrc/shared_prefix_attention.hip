@@ -198,7 +198,7 @@ struct Share {
 typedef const __attribute__((address_space(4))) int* scalar_ints;  // uniform reads go through the scalar unit
 
 // The block of a table's entry. Entries that hold none may be any negative number: they lead to block 0 and not outside the pools
-// where a group is said to share more keys than its table has (a max a table entry costs nothing measurable).
+// where a group is said to share more keys than its table has (the max is taken where an entry is used: at its load, a step ahead, it would wait for it).
 __device__ __forceinline__ int block_at(int entry) { return max(entry, 0); }
 
 // ---- many rows: the waves share tiles of K and V in LDS, 32 rows a wave ---------------------------
@@ -232,7 +232,7 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
     // A wave brings half a tile's K or V, 16 keys of one table entry, which it looks up a tile ahead.
     int entry;
     const auto first16 = [&](int j) { return min(g.begin + j * kStep + 16 * (w & 1), (g.end - 1) & ~15); };
-    const auto lookup = [&](int j) { entry = block_at(entries[first16(j) >> sh]); };
+    const auto lookup = [&](int j) { entry = entries[first16(j) >> sh]; };
     uint32_t piece[PER16];  // a lane's offsets in 16 keys
     const auto pieces_to = [&](int last) {
 #pragma unroll
@@ -244,7 +244,7 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
     pieces_to(15);
     const auto send = [&](int j, int slot) {
       const int key = first16(j);
-      const half_t* const base = pool + ((static_cast<int64_t>(entry) * a.kv_heads + g.kvh) * bs + (key & (bs - 1))) * D;
+      const half_t* const base = pool + ((static_cast<int64_t>(block_at(entry)) * a.kv_heads + g.kvh) * bs + (key & (bs - 1))) * D;
       if (g.end - key < 16) pieces_to(g.end - 1 - key);  // the last tile: past the end the last key again
 #pragma unroll
       for (int i = 0; i < PER16; ++i)
@@ -435,12 +435,12 @@ __device__ __forceinline__ void attend_few(const SharedArgs& a, Share sh, char* 
     int entry[2];
     const auto run_of = [&](int k0, int t) { return min(k0 + 16 * t, (end - 1) & ~15); };
     const auto lookup = [&](int k0) {
-      if (SCALAR) entry[0] = block_at(entries[run_of(k0, 0) >> bshift]), entry[1] = block_at(entries[run_of(k0, 1) >> bshift]);
+      if (SCALAR) entry[0] = entries[run_of(k0, 0) >> bshift], entry[1] = entries[run_of(k0, 1) >> bshift];
     };
     const auto issue = [&](KvStep<D, DR>& st, int k0) {
       const auto row_of = [&](int t, int off) -> unsigned {
         const int r0 = run_of(k0, t);
-        return (static_cast<unsigned>(entry[t]) * a.kv_heads + sh.kvh) * bs + (r0 & (bs - 1)) + min(max(off, begin - r0), end - 1 - r0);
+        return (static_cast<unsigned>(block_at(entry[t])) * a.kv_heads + sh.kvh) * bs + (r0 & (bs - 1)) + min(max(off, begin - r0), end - 1 - r0);
       };
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
