@@ -11,14 +11,14 @@
 //
 //  - many rows (prefixes of more than 16 rows or 1024 keys, or of more than 12 rows of 128): 128 rows, 32 a
 //    wave, on tiles of K and V that the waves share in LDS (attend_rows). 64 x 4 rows on 16,384 keys of
-//    8 heads of 128 (17 GFLOP, 67 MB) take 40 us, the join of their 16 slices 8. Bound by the chain of a
+//    8 heads of 128 (17 GFLOP, 67 MB) take 41 us, the join of their slices 6. Bound by the chain of a
 //    step (LDS reads, products, weights: no one of them taken out made it faster by over a tenth); a
 //    ring of five tiles takes 5-10% longer.
 //  - few rows (own keys, short prefixes): 16 rows, the waves on keys of their own, K straight into MFMA
 //    operands (attend_few). Bound by memory: 64 x 1000 own keys, 8 kv heads of 128 (ragged, 164 MB) 34 us.
 //
 // One launch does both, prefixes first: the prefix's products run beside the own keys' loads. 64 members on
-// 16,384 keys with up to 1000 of their own (231 MB, 18 GFLOP) take 58 us, the join 5.5. Prefix tiles staged
+// 16,384 keys with up to 1000 of their own (231 MB, 18 GFLOP) take 60 us, the join 5.9. Prefix tiles staged
 // through registers, whose reloads from scratch waited for every load in flight, took 107 in all, and
 // workgroups of eight waves that do not share their tiles 244.
 #include <algorithm>
@@ -385,7 +385,9 @@ __device__ __forceinline__ void attend_rows(const SharedArgs& a, Share g, char* 
 //
 // with lane (c, g) on row c and keys 4 g .. 4 g + 3 of each 16. K goes straight into MFMA operands, V through a
 // staging area of the wave in LDS, and the loads of the next step are in flight under this one's work,
-// so that a workgroup alone on its CU, as at the end of a batch of ragged lengths, still streams.
+// so that a workgroup alone on its CU, as at the end of a batch of ragged lengths, still streams. That holds up to head size
+// 64. At 128 two steps' operands pass the 256 registers by 16 (by 26 where blocks are no power of two from 16 on), and what is
+// spilled in the loop is stored and fetched behind waits for all loads: every second step waits for the loads it should overlap.
 template <int D, int DR>
 struct KvStep {
   half8 k[2][D / 32], v[kStep * (D / 8) / kWave];

@@ -378,12 +378,13 @@ struct QkArgs {
   Div by_block, by_sets;  // by_sets: sets of heads a token
 };
 
-// PLAIN: one plane and no scale, without the branches of up to 8 (2047 rows of 32/4 heads of 64 9.6 us, with them 10.9).
+// PLAIN: one plane and no scale, without the branches of up to 8 (2047 rows of 32/4 heads of 64 9.6 us, with them
+// 10.8, one row 3.1 and 3.8; these figures and those below in a graph, call after call).
 template <int LANES, int HEADS, bool PLAIN>
 __global__ __launch_bounds__(kThreads) void qk_norm_kernel(const QkArgs a) {
   constexpr int PER = kWave / LANES;  // heads of a set
   // The arguments at once: the compiler loads them where they are used, one wait after another (2047 rows of 32/4
-  // heads of 64 10.4 -> 9.4 us; the tables' and the logits' kernels gain nothing by it).
+  // heads of 64 10.4 -> 9.6 us; the tables' and the logits' kernels gain nothing by it).
   asm volatile("" : : "s"(a.qkv), "s"(a.planes), "s"(a.scale), "s"(a.T), "s"(a.bias), "s"(a.q_norm), "s"(a.k_norm), "s"(a.eps), "s"(a.inv_freq),
                "s"(a.pos), "s"(a.slot), "s"(a.kpool), "s"(a.vpool), "s"(a.q_out), "s"(a.q_scale), "s"(a.heads), "s"(a.kv_heads), "s"(a.D),
                "s"(a.block), "s"(a.by_block.m), "s"(a.by_sets.m));
@@ -521,13 +522,13 @@ template <bool BIAS, bool VEC, int kVec, int THREADS>
 __global__ __launch_bounds__(THREADS) void process_logits_kernel(const LogitArgs a) {
   // A word for each logit of the slice: first what the history says, then the last bias that names it
   // (an array of its own for these would halve the workgroups that a CU holds: 64 rows of 128,257
-  // 32 / 30 us).
+  // then 32 / 30 us).
   constexpr int kSlice = 4 * kVec * THREADS;
   __shared__ __attribute__((aligned(16))) unsigned s_word[kSlice];
   __shared__ unsigned long long s_best[THREADS / 64];
   __shared__ int s_last;
   // Workgroups go round the 8 XCDs; a row's go to one, whose L2 then serves its history (as many rows as come in
-  // eights; 64 rows of 32,000 with histories of 8000 15 / 13.8 us, of 128,257 with 100 level).
+  // eights; 64 rows of 32,000 with histories of 8000 12.7 / 11.1 us, of 128,257 with 8000 27.0 / 26.2, with 100 level).
   int row = blockIdx.x / a.slices, part = blockIdx.x % a.slices;
   if (row < (a.rows & ~7)) {
     const int over = (blockIdx.x >> 3) / a.slices;
@@ -732,7 +733,8 @@ int slice_of(int rows, int vocab, int threads) {
 int slices_of(int vocab, int slice) { return static_cast<int>((static_cast<int64_t>(vocab) + 3 + slice - 1) / slice); }
 
 // A row's record has 256-byte lines of its own: counts of several rows in one line are taken one after
-// another, 10 ns each (64 rows of 128,257 logits 37 us, with a line each 32).
+// another, 10 ns each (with all counts side by side 64 rows of 128,257 logits took 37 us, with a line each 32; in records of a
+// row's own without whole lines they are level with this).
 int64_t record_words(int vocab, int slice) { return (1 + static_cast<int64_t>(slices_of(vocab, slice)) + 31) / 32 * 32; }
 
 }  // namespace
@@ -809,8 +811,8 @@ int rh_qk_norm_to_cache(const float* qkv, int planes, const float* scale, int T,
     };
     constexpr int PER = kWave / LANES;
     // Two sets of heads a wave once that leaves enough waves. Measured (us, one / two; bound by latency
-    // below, by memory above): 48 rows of 32/4 heads of 64 3.2 / 3.6, 256 3.6 / 3.7, 512 4.3 / 4.3, 2047 10.3 /
-    // 9.6 (floor 6.1), 4096 of 32/8 heads of 128 37 / 33 (29); three to five sets are level.
+    // below, by memory above): 48 rows of 32/4 heads of 64 3.2 / 3.6, 256 3.6 / 3.7, 512 4.2 / 4.3, 2047 10.2 /
+    // 9.6 (floor 6.1), 4096 of 32/8 heads of 128 37.5 / 32.5 (29); three to five sets are level.
     const bool many = static_cast<int64_t>(T) * total * LANES >= 150000;
     if (planes == 1 && !scale) return many ? go(qk_norm_kernel<LANES, 2, true>, 2 * PER) : go(qk_norm_kernel<LANES, 1, true>, PER);
     return many ? go(qk_norm_kernel<LANES, 2, false>, 2 * PER) : go(qk_norm_kernel<LANES, 1, false>, PER);
