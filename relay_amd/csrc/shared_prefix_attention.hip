@@ -787,6 +787,7 @@ struct Plan {
 Plan plan_of(int n_dec, int n_groups, int max_members, int max_shared, int max_own, int heads, int kv_heads, int head_dim,
              int block) {
   const int group = heads / kv_heads;
+  max_members = std::min(max_members, n_dec);  // a group has no more, whatever the caller allows for
   const int64_t rows = static_cast<int64_t>(max_members) * group;
   Plan p{};
   // Shared tiles come in pieces of up to 16 keys of one block, straight to LDS.

@@ -34,6 +34,11 @@ def run(torch, dev, case, tol_of, **kw):
             assert (off <= tol).all(), f"row {row}, head {h}: off by {off.max()}, {np.max(off / tol)} of the tolerance"
 
 
+def usual(D):
+    """The tolerance of any keys: the weights' rounding besides, and scores summed in fp32."""
+    return lambda o, a, c, v, size: equal_weights(o, a, c, v, size) + c * 2.0 ** -36 * v + 2 * (D + 2) * 2.0 ** -24 * size * a
+
+
 def equal_weights(o, a, c, v, size):
     """Of keys whose scores are equal or too far apart to count: the weights' rounding to fp16, the sums' at most 64 roundings of 2^-24 and the
     result's to fp16, 2^-11 (2^-25 where it is subnormal)."""
@@ -145,3 +150,11 @@ def test_no_groups_at_all(torch_mod, dev, D):
     _lib.check(call.lib.rh_shared_prefix_attention(*args, None))
     torch_mod.cuda.synchronize()
     assert (np.abs(call.out.double().cpu().numpy() - want) <= tol).all()
+
+
+@gpu
+@pytest.mark.parametrize("hints", [(2 ** 31 - 1, 2000, 300), (65536, 1 << 30, 1 << 30)])
+@pytest.mark.parametrize("heads,kv_heads,D", [(32, 8, 128), (9, 3, 64)])
+def test_hints_far_above_many_groups(torch_mod, dev, heads, kv_heads, D, hints):
+    """A group has no more members than there are tokens: the largest numbers that the call takes for its sizes fit its launch."""
+    run(torch_mod, dev, Case([(3, 160 + 16 * (i % 5)) for i in range(40)], [9, 40], heads, kv_heads, D, seed=D), usual(D), hints=hints)
