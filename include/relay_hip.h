@@ -556,7 +556,7 @@ size_t rh_shared_prefix_workspace(int n_dec, int n_groups, int max_members, int 
 
 /* 1 where sharing should be faster than rh_paged_decode_attention on the same dec_meta (whose fourth
  * values that ignores) and tables, if every token's own table holds its whole context: a rule from
- * timings of 2000 shapes, right in 97 of 100 that it answers with 1 (groups of two are most of the rest).
+ * timings of 2000 shapes, right in 96 of 100 that it answers with 1 (a third of the others are groups of two).
  * 0 for one token, which shares nothing. */
 int rh_shared_prefix_pays(int n_dec, int max_shared, int max_own, int heads, int kv_heads, int head_dim);
 
